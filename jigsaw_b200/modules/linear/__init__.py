@@ -22,8 +22,10 @@ from ._linear import (
     MatMulXW,
     MatMulXWT,
 )
+from ._scaled import BlockScaled, quantize_blockwise, scaled_linear, scaled_matmul
 
 __all__ = [
+    "BlockScaled",
     "DistributedLinear",
     "DistributedMatMulXTW",
     "DistributedMatMulXW",
@@ -32,6 +34,9 @@ __all__ = [
     "MatMulXTW",
     "MatMulXW",
     "MatMulXWT",
+    "quantize_blockwise",
+    "scaled_linear",
+    "scaled_matmul",
 ]
 
 set_module(globals(), __all__)

@@ -1,0 +1,264 @@
+"""Root-mean-square norm with the residual's addition, in the input's type, in 8 bits, and fused in front of an 8-bit
+linear layer.
+
+    t = x + residual            (rounded to the type of x: the sum is stored, and the norm is of the stored sum)
+    y = t * r * weight,         r = (mean(t^2) + eps)^(-1/2)
+
+    dt_k = r (w_k g_k - r^2 t_k mean(w g t)) + gradient that reaches the sum on its own,    dw = sum over rows of g t r
+
+The feature axis may be cut over a column group: the sum of squares is then added over the group (a differentiable
+all-reduce, whose adjoint is the backward pass's).
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Any
+
+import torch
+import torch.distributed as dist
+from torch.autograd.function import once_differentiable
+
+from ..._core.autocast import autocast_dtype
+from ..._core.collectives import all_reduce_sum
+from ..linear._scaled import (
+    _HALF,
+    ROW,
+    SQUARE,
+    BlockScaled,
+    _check_linear,
+    _grads,
+    _product,
+    _quantize_2d,
+    _quantize_plain,
+    _refuse_vmap,
+)
+
+
+def _check(name: str, x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None, eps: float) -> None:
+    if not x.is_floating_point() or x.element_size() == 1:
+        raise TypeError(f"{name} takes fp64, fp32, bf16 or fp16 tensors, got {x.dtype}")
+    if x.dim() == 0:
+        raise ValueError(f"{name} needs at least one dimension")
+    if weight is not None and weight.shape != (x.shape[-1],):
+        raise ValueError(f"{name}: weight of shape {tuple(weight.shape)} for {x.shape[-1]} features")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"{name}: residual of shape {tuple(residual.shape)}, input of shape {tuple(x.shape)}")
+    for t in (weight, residual):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name}: input on {x.device}, weight or residual on {t.device}")
+    if not (math.isfinite(eps) and eps >= 0):
+        raise ValueError(f"{name}: eps must be finite and not negative, got {eps}")
+
+
+def _same_type(x: torch.Tensor, residual: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    if residual is None or residual.dtype == x.dtype:
+        return x, residual
+    dt = torch.promote_types(x.dtype, residual.dtype)
+    return x.to(dt), residual.to(dt)
+
+
+def _plain(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None, col_group: Any, eps: float) -> tuple:
+    """``(normalised rows in fp32 or wider, sum, r)`` in torch operations."""
+    t = x if residual is None else x + residual
+    wide = t.to(torch.promote_types(t.dtype, torch.float32))
+    parts = 1 if col_group is None else col_group.size()
+    sq = (wide * wide).sum(dim=-1, keepdim=True)
+    if parts > 1:
+        sq = all_reduce_sum(sq, col_group)
+    r = torch.rsqrt(sq / (wide.shape[-1] * parts) + eps)
+    y = wide * r
+    return (y if weight is None else y * weight.to(torch.promote_types(weight.dtype, wide.dtype))), t, r
+
+
+class _FusedRmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None, eps: float,
+                out_dtype: torch.dtype, need: bool) -> Any:
+        from ...ops import scaled_fused
+
+        y, _, _, total, rstd = scaled_fused.maybe_fused_rms_norm(x, weight, eps, residual, out_dtype, False, need)
+        ctx.set_materialize_grads(False)
+        ctx.has_residual = residual is not None
+        if need:
+            ctx.save_for_backward(x if total is None else total, weight, rstd)
+        return y if total is None else (y, total)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, g: torch.Tensor | None, gsum: torch.Tensor | None = None) -> tuple:
+        t, weight, rstd = ctx.saved_tensors
+        dx, dw = _norm_backward(t, weight, rstd, g, gsum, ctx.needs_input_grad[1])
+        return dx, dw, dx if ctx.has_residual else None, None, None, None
+
+
+def _norm_backward(t: torch.Tensor, weight: torch.Tensor | None, rstd: torch.Tensor, g: torch.Tensor | None,
+                   gsum: torch.Tensor | None, want_w: bool) -> tuple:
+    """Gradients of the sum and of the weight; ``rstd [R]`` as the forward pass computed it."""
+    want_w = want_w and weight is not None
+    if g is None:                                 # only the sum was used
+        return (None if gsum is None else gsum.to(t.dtype)), (torch.zeros_like(weight) if want_w and weight is not None else None)
+    if t.is_cuda:
+        from ...ops import scaled_fused
+
+        if g.dtype not in (t.dtype, torch.float32):
+            g = g.float()
+        return scaled_fused.rms_norm_backward(t, rstd, weight, g, gsum, want_w)
+    tw, gw, r = t.float(), g.float(), rstd[:, None]
+    gy = gw if weight is None else gw * weight.float()
+    dx = r * (gy - tw * (r * r * (gy * tw).mean(dim=1, keepdim=True)))
+    if gsum is not None:
+        dx = dx + gsum.float()
+    return dx.to(t.dtype), (gw * tw * r).sum(dim=0).to(weight.dtype) if want_w and weight is not None else None
+
+
+def _rows(t: torch.Tensor | None, c: int) -> torch.Tensor | None:
+    return t if t is None or t.dim() == 2 else t.reshape(-1, c)
+
+
+def distributed_rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, col_group: dist.ProcessGroup | None = None,
+                         eps: float = 1e-6, residual: torch.Tensor | None = None) -> Any:
+    """Root-mean-square norm of the last axis of ``x`` (cut over ``col_group``), times ``weight``.
+
+    With ``residual`` (same shape) the norm is of ``x + residual``, and ``(y, x + residual)`` is returned: the sum, in the
+    common type of the two, is the residual of the next block.  Statistics are fp32 or wider; ``y`` is fp32 under autocast
+    and has the type of the sum otherwise.  Differentiable in every tensor.  On CUDA with the whole feature axis on one
+    rank, fp32, bf16 and fp16 run as one kernel per direction (plus one that adds up the weight's gradient)."""
+    _check("distributed_rms_norm", x, weight, residual, eps)
+    x, residual = _same_type(x, residual)
+    c = x.shape[-1]
+    out_dtype = x.dtype if autocast_dtype(x.device.type) is None else torch.promote_types(x.dtype, torch.float32)
+    whole = col_group is None or col_group.size() == 1
+    if x.is_cuda and whole and _fusable(x, weight, c):
+        need = any(_grads(x, weight, residual))
+        out = _FusedRmsNorm.apply(_rows(x, c), weight, _rows(residual, c), eps, out_dtype, need)
+        if residual is None:
+            return out.view(x.shape)
+        return out[0].view(x.shape), out[1].view(x.shape)
+    y, t, _ = _plain(x, weight, residual, col_group, eps)
+    y = y.to(out_dtype)
+    return y if residual is None else (y, t)
+
+
+def _fusable(x: torch.Tensor, weight: torch.Tensor | None, c: int) -> bool:
+    if x.numel() == 0 or x.dtype not in _HALF or (weight is not None and weight.dtype not in _HALF):
+        return False
+    if torch._C._functorch.is_batchedtensor(x) or (weight is not None and torch._C._functorch.is_batchedtensor(weight)):
+        return False
+    from ...ops import _lib
+
+    if not _lib.available():
+        raise RuntimeError("jigsaw_b200: the sm_100a kernel library is missing on a CUDA machine")
+    return c <= _lib.lib().jb_rms_max_cols()
+
+
+def _norm_to_codes(x: torch.Tensor, weight: torch.Tensor | None, eps: float, residual: torch.Tensor | None,
+                   keep_rstd: bool) -> tuple[BlockScaled, torch.Tensor, torch.Tensor | None]:
+    """``(codes, sum, r)`` of matrices."""
+    if x.is_cuda:
+        from ...ops import scaled_fused
+
+        out = scaled_fused.maybe_fused_rms_norm(x, weight, eps, residual, None, True, keep_rstd)
+        if out is not None:
+            return BlockScaled(out[1], out[2], ROW), (x if out[3] is None else out[3]), out[4]
+    y, t, r = _plain(x, weight, residual, None, eps)
+    return BlockScaled(*_quantize_plain(y, ROW), ROW), t, r.squeeze(-1)
+
+
+def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6,
+                      residual: torch.Tensor | None = None) -> Any:
+    """Root-mean-square norm with the output in 8 bits (blocks of 128 features, quantised from the unrounded fp32 value):
+    a :class:`BlockScaled`, or ``(BlockScaled, x + residual)`` with a residual.  For inference: not differentiable
+    (:func:`rms_norm_linear` is), so tensors that want gradients are refused."""
+    _check("rms_norm_quantize", x, weight, residual, eps)
+    _refuse_vmap("rms_norm_quantize", x, weight, residual)
+    if any(_grads(x, weight, residual)):
+        raise ValueError("rms_norm_quantize has no gradient; use rms_norm_linear, or call it under torch.no_grad()")
+    x, residual = _same_type(x, residual)
+    c = x.shape[-1]
+    if x.numel() == 0:
+        empty = BlockScaled(x.new_empty(x.shape, dtype=torch.float8_e4m3fn),
+                            x.new_empty((*x.shape[:-1], -(-c // 128)), dtype=torch.float8_e8m0fnu), ROW)
+        return empty if residual is None else (empty, x + residual)
+    flat = x.reshape(-1, c)
+    q, t, _ = _norm_to_codes(flat.detach(), weight, eps, None if residual is None else residual.detach().reshape(-1, c), False)
+    if x.dim() == 1:
+        q = BlockScaled(q.codes[0], q.scales[0], ROW)
+    elif x.dim() > 2:
+        q = BlockScaled(q.codes.unflatten(0, x.shape[:-1]), q.scales.unflatten(0, x.shape[:-1]), ROW)
+    return q if residual is None else (q, t.view(x.shape))
+
+
+class _RmsNormLinear(torch.autograd.Function):
+    """Norm, quantisation and product in two launches (three with the weight's quantisation); the normalised rows exist
+    only as codes.  The backward pass recomputes them from the stored sum, straight into the column blocks that the weight
+    gradient wants, and keeps the gradient of the normalised rows in fp32 between the product and the norm."""
+
+    @staticmethod
+    def forward(ctx: Any, x: torch.Tensor, gain: torch.Tensor | None, w: torch.Tensor, b: torch.Tensor | None, eps: float,
+                residual: torch.Tensor | None, out_dtype: torch.dtype, need_h: bool, need_w: bool) -> Any:
+        q, t, r = _norm_to_codes(x, gain, eps, residual, need_h or need_w)
+        wr, wc, _ = _quantize_2d(w, SQUARE, cols=need_h)
+        ctx.set_materialize_grads(False)
+        ctx.need_w, ctx.has_residual = need_w, residual is not None
+        ctx.types = (w.dtype, None if b is None else b.dtype)
+        if need_h or need_w:
+            ctx.save_for_backward(t, r, gain, *((wc.codes, wc.scales) if wc is not None else (None, None)))
+        y = _product(q, wr, b, out_dtype)
+        return y if residual is None else (y, t)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, g: torch.Tensor | None, gsum: torch.Tensor | None = None) -> tuple:
+        want_b = ctx.needs_input_grad[3] and ctx.types[1] is not None
+        if not ctx.saved_tensors:                 # only the bias wants a gradient
+            db = g.sum(dim=0, dtype=torch.float32).to(ctx.types[1]) if g is not None and want_b else None
+            return (None, None, None, db) + (None,) * 5
+        t, r, gain, wc, ws = ctx.saved_tensors
+        dh = dw = db = None
+        if g is not None:
+            gr, gc, db = _quantize_2d(g, ROW, rows=wc is not None, cols=ctx.need_w, colsum=ctx.types[1] if want_b else None)
+            if wc is not None:
+                dh = _product(gr, BlockScaled(wc, ws, SQUARE), None, torch.float32)
+            if ctx.need_w:
+                hc = _quantize_2d(t, ROW, rows=False, cols=True, rstd=r, gain=gain)[1]
+                dw = _product(gc, hc, None, ctx.types[0])
+        dx, dgain = _norm_backward(t, gain, r, dh, gsum, ctx.needs_input_grad[1])
+        return dx, dgain, dw, db, None, dx if ctx.has_residual else None, None, None, None
+
+
+def rms_norm_linear(x: torch.Tensor, norm_weight: torch.Tensor | None, weight: "torch.Tensor | BlockScaled",
+                    bias: torch.Tensor | None = None, eps: float = 1e-6, residual: torch.Tensor | None = None) -> Any:
+    """``scaled_linear(rms_norm(x + residual) , weight, bias)`` with the norm's output in 8 bits from the start: the
+    normalised rows are quantised from their unrounded fp32 values and never stored otherwise.  Returns ``y``, or
+    ``(y, x + residual)`` with a residual.  Differentiable like :func:`scaled_linear`; a prepared ``weight`` serves
+    inference."""
+    K, N, prepared = _check_linear("rms_norm_linear", x, weight, bias)
+    _check("rms_norm_linear", x, norm_weight, residual, eps)
+    _refuse_vmap("rms_norm_linear", norm_weight, residual)
+    if (norm_weight is not None and norm_weight.dtype not in _HALF) or (residual is not None and residual.dtype not in _HALF):
+        raise TypeError("rms_norm_linear takes fp32, bf16 or fp16 tensors")
+    if prepared and any(_grads(norm_weight, residual)):
+        raise ValueError("rms_norm_linear: a prepared weight (BlockScaled) serves inference only; call it under torch.no_grad()")
+    out_dtype = autocast_dtype(x.device.type) or x.dtype
+    x, residual = _same_type(x, residual)
+    if out_dtype not in _HALF:
+        out_dtype = x.dtype
+    M = math.prod(x.shape[:-1])
+    if M == 0 or N == 0 or K == 0:
+        h, t, _ = _plain(x, norm_weight, residual, None, eps)
+        w = weight.dequantize() if prepared else weight.float()
+        y = torch.nn.functional.linear(h.float(), w, None if bias is None else bias.float()).to(out_dtype)
+        return y if residual is None else (y, t)
+    x2, r2 = _rows(x, K), _rows(residual, K)
+    if x2.dim() == 1:
+        x2, r2 = x2[None], None if r2 is None else r2[None]
+    if prepared:
+        q, t, _ = _norm_to_codes(x2.detach(), norm_weight, eps, None if r2 is None else r2.detach(), False)
+        y = _product(q, weight, None if bias is None else bias.detach(), out_dtype)
+    else:
+        gx, gn, gw, gr = _grads(x, norm_weight, weight, residual)
+        out = _RmsNormLinear.apply(x2, norm_weight, weight, bias, eps, r2, out_dtype, gx or gn or gr, gw)
+        y, t = (out, None) if residual is None else out
+    y = y.view(*x.shape[:-1], N)
+    return y if residual is None else (y, t.view(x.shape))

@@ -13,5 +13,7 @@
 #include "allreduce.cu"
 #include "flash_attn.cu"
 #include "flash_attn_bwd.cu"
+#include "scaled_quant.cu"
+#include "scaled_gemm.cu"
 
 extern "C" int jb_abi_version() { return 1; }
