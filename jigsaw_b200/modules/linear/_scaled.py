@@ -124,26 +124,17 @@ def _quantize_2d(x: torch.Tensor, block: tuple[int, int], rows: bool = True, col
 
 
 def _product(a: BlockScaled, b: BlockScaled, bias: torch.Tensor | None, out_dtype: torch.dtype) -> torch.Tensor:
-    """``a [M, K] b [N, K]^T + bias``."""
+    """``a [..., K] b [N, K]^T + bias``."""
     if a.codes.is_cuda:
         from ...ops import scaled_fused
 
-        out = scaled_fused.maybe_fused_scaled_matmul(a.codes, a.scales, a.block == SQUARE, b.codes, b.scales, b.block == SQUARE,
-                                                     bias, out_dtype)
+        out = scaled_fused.maybe_fused_scaled_matmul(a, b, bias, out_dtype)
         if out is not None:
             return out
     y = a.dequantize() @ b.dequantize().t()
     if bias is not None:
         y = y + bias.float()
     return y.to(out_dtype)
-
-
-def _flat(q: BlockScaled) -> BlockScaled:
-    if q.codes.dim() == 2:
-        return q
-    # the row count is spelt out: -1 cannot be inferred for an empty operand
-    rows = math.prod(q.codes.shape[:-1])
-    return BlockScaled(q.codes.reshape(rows, q.codes.shape[-1]), q.scales.reshape(rows, q.scales.shape[-1]), q.block)
 
 
 # ----------------------------------------------------------------------------- public functions
@@ -211,14 +202,13 @@ def scaled_matmul(a: BlockScaled, b: BlockScaled, bias: torch.Tensor | None = No
     if a.codes.numel() == 0 or n == 0:
         y = torch.zeros(*a.shape[:-1], n, dtype=torch.float32, device=a.codes.device)
         return (y if bias is None else y + bias.detach().float()).to(out_dtype)
-    y = _product(_flat(a), b, None if bias is None else bias.detach(), out_dtype)
-    return y if a.codes.dim() == 2 else y.view(*a.shape[:-1], n)
+    return _product(a, b, None if bias is None else bias.detach(), out_dtype)
 
 
 class _ScaledLinear(torch.autograd.Function):
     """``y = q(x) q(w)^T + b`` and its gradients as two more 8-bit products: ``dx = q(g) q(w)`` with blocks of ``g`` along the
-    output features, ``dw = q(g^T) q(x^T)^T`` with blocks of both along the tokens.  Each operand is read once and written in
-    the two layouts that the products want."""
+    output features, ``dw = q(g^T) q(x^T)^T`` with blocks of both along the tokens.  (CUDA calls take the native form of the
+    same function.)"""
 
     @staticmethod
     def forward(ctx: Any, x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, out_dtype: torch.dtype, need_x: bool,
@@ -293,11 +283,19 @@ def scaled_linear(x: torch.Tensor, weight: "torch.Tensor | BlockScaled", bias: t
     if M == 0 or N == 0 or K == 0:
         w = weight.dequantize(x.dtype) if prepared else weight.to(x.dtype)
         return torch.nn.functional.linear(x, w, None if bias is None else bias.to(x.dtype)).to(out_dtype)
-    x2 = x if x.dim() == 2 else x.reshape(M, K)
     if prepared:
-        q = _quantize_2d(x2.detach(), ROW)[0]
-        y = _product(q, weight, None if bias is None else bias.detach(), out_dtype)
-    else:
-        need_x, need_w = _grads(x, weight)
-        y = _ScaledLinear.apply(x2, weight, bias, out_dtype, need_x, need_w)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+        b = None if bias is None else bias.detach()
+        if x.is_cuda:
+            from ...ops import scaled_fused
+
+            return scaled_fused.prepared_linear(x.detach(), weight, b, out_dtype)
+        return _product(quantize_blockwise(x), weight, b, out_dtype)
+    need_x, need_w = _grads(x, weight)
+    if x.is_cuda:
+        from ...ops import scaled_fused
+
+        out = scaled_fused.maybe_fused_scaled_linear(x, weight, bias, out_dtype, need_x, need_w)
+        if out is not None:
+            return out
+    y = _ScaledLinear.apply(x.reshape(M, K), weight, bias, out_dtype, need_x, need_w)
+    return y.view(*x.shape[:-1], N)

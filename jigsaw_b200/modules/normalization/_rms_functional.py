@@ -30,8 +30,8 @@ from ..linear._scaled import (
     _grads,
     _product,
     _quantize_2d,
-    _quantize_plain,
     _refuse_vmap,
+    quantize_blockwise,
 )
 
 
@@ -71,49 +71,18 @@ def _plain(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor 
     return (y if weight is None else y * weight.to(torch.promote_types(weight.dtype, wide.dtype))), t, r
 
 
-class _FusedRmsNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx: Any, x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None, eps: float,
-                out_dtype: torch.dtype, need: bool) -> Any:
-        from ...ops import scaled_fused
-
-        y, _, _, total, rstd = scaled_fused.maybe_fused_rms_norm(x, weight, eps, residual, out_dtype, False, need)
-        ctx.set_materialize_grads(False)
-        ctx.has_residual = residual is not None
-        if need:
-            ctx.save_for_backward(x if total is None else total, weight, rstd)
-        return y if total is None else (y, total)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, g: torch.Tensor | None, gsum: torch.Tensor | None = None) -> tuple:
-        t, weight, rstd = ctx.saved_tensors
-        dx, dw = _norm_backward(t, weight, rstd, g, gsum, ctx.needs_input_grad[1])
-        return dx, dw, dx if ctx.has_residual else None, None, None, None
-
-
 def _norm_backward(t: torch.Tensor, weight: torch.Tensor | None, rstd: torch.Tensor, g: torch.Tensor | None,
                    gsum: torch.Tensor | None, want_w: bool) -> tuple:
     """Gradients of the sum and of the weight; ``rstd [R]`` as the forward pass computed it."""
     want_w = want_w and weight is not None
     if g is None:                                 # only the sum was used
         return (None if gsum is None else gsum.to(t.dtype)), (torch.zeros_like(weight) if want_w and weight is not None else None)
-    if t.is_cuda:
-        from ...ops import scaled_fused
-
-        if g.dtype not in (t.dtype, torch.float32):
-            g = g.float()
-        return scaled_fused.rms_norm_backward(t, rstd, weight, g, gsum, want_w)
     tw, gw, r = t.float(), g.float(), rstd[:, None]
     gy = gw if weight is None else gw * weight.float()
     dx = r * (gy - tw * (r * r * (gy * tw).mean(dim=1, keepdim=True)))
     if gsum is not None:
         dx = dx + gsum.float()
     return dx.to(t.dtype), (gw * tw * r).sum(dim=0).to(weight.dtype) if want_w and weight is not None else None
-
-
-def _rows(t: torch.Tensor | None, c: int) -> torch.Tensor | None:
-    return t if t is None or t.dim() == 2 else t.reshape(-1, c)
 
 
 def distributed_rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, col_group: dist.ProcessGroup | None = None,
@@ -126,43 +95,35 @@ def distributed_rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, co
     rank, fp32, bf16 and fp16 run as one kernel per direction (plus one that adds up the weight's gradient)."""
     _check("distributed_rms_norm", x, weight, residual, eps)
     x, residual = _same_type(x, residual)
-    c = x.shape[-1]
     out_dtype = x.dtype if autocast_dtype(x.device.type) is None else torch.promote_types(x.dtype, torch.float32)
     whole = col_group is None or col_group.size() == 1
-    if x.is_cuda and whole and _fusable(x, weight, c):
-        need = any(_grads(x, weight, residual))
-        out = _FusedRmsNorm.apply(_rows(x, c), weight, _rows(residual, c), eps, out_dtype, need)
-        if residual is None:
-            return out.view(x.shape)
-        return out[0].view(x.shape), out[1].view(x.shape)
+    if x.is_cuda and whole and _fusable(x, weight, residual):
+        from ...ops import scaled_fused
+
+        out = scaled_fused.maybe_fused_rms_norm(x, weight, residual, eps, out_dtype, any(_grads(x, weight, residual)))
+        if out is not None:
+            return out[0] if residual is None else out
     y, t, _ = _plain(x, weight, residual, col_group, eps)
     y = y.to(out_dtype)
     return y if residual is None else (y, t)
 
 
-def _fusable(x: torch.Tensor, weight: torch.Tensor | None, c: int) -> bool:
-    if x.numel() == 0 or x.dtype not in _HALF or (weight is not None and weight.dtype not in _HALF):
-        return False
-    if torch._C._functorch.is_batchedtensor(x) or (weight is not None and torch._C._functorch.is_batchedtensor(weight)):
-        return False
-    from ...ops import _lib
-
-    if not _lib.available():
-        raise RuntimeError("jigsaw_b200: the sm_100a kernel library is missing on a CUDA machine")
-    return c <= _lib.lib().jb_rms_max_cols()
+def _fusable(*tensors: torch.Tensor | None) -> bool:
+    """Types that the kernels take, at least one element, no ``torch.vmap`` (the kernels have no batching rules)."""
+    return all(t is None or (t.dtype in _HALF and t.numel() > 0 and not torch._C._functorch.is_batchedtensor(t)) for t in tensors)
 
 
 def _norm_to_codes(x: torch.Tensor, weight: torch.Tensor | None, eps: float, residual: torch.Tensor | None,
                    keep_rstd: bool) -> tuple[BlockScaled, torch.Tensor, torch.Tensor | None]:
-    """``(codes, sum, r)`` of matrices."""
-    if x.is_cuda:
+    """``(codes, sum, r)``; ``r`` per row."""
+    if x.is_cuda and _fusable(x, weight, residual):
         from ...ops import scaled_fused
 
-        out = scaled_fused.maybe_fused_rms_norm(x, weight, eps, residual, None, True, keep_rstd)
+        out = scaled_fused.maybe_fused_rms_quantize(x, weight, eps, residual, keep_rstd)
         if out is not None:
-            return BlockScaled(out[1], out[2], ROW), (x if out[3] is None else out[3]), out[4]
+            return BlockScaled(out[0], out[1], ROW), (x if out[2] is None else out[2]), out[3]
     y, t, r = _plain(x, weight, residual, None, eps)
-    return BlockScaled(*_quantize_plain(y, ROW), ROW), t, r.squeeze(-1)
+    return quantize_blockwise(y), t, r.reshape(-1)
 
 
 def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6,
@@ -180,19 +141,14 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, eps: 
         empty = BlockScaled(x.new_empty(x.shape, dtype=torch.float8_e4m3fn),
                             x.new_empty((*x.shape[:-1], -(-c // 128)), dtype=torch.float8_e8m0fnu), ROW)
         return empty if residual is None else (empty, x + residual)
-    flat = x.reshape(-1, c)
-    q, t, _ = _norm_to_codes(flat.detach(), weight, eps, None if residual is None else residual.detach().reshape(-1, c), False)
-    if x.dim() == 1:
-        q = BlockScaled(q.codes[0], q.scales[0], ROW)
-    elif x.dim() > 2:
-        q = BlockScaled(q.codes.unflatten(0, x.shape[:-1]), q.scales.unflatten(0, x.shape[:-1]), ROW)
-    return q if residual is None else (q, t.view(x.shape))
+    q, t, _ = _norm_to_codes(x.detach(), weight, eps, None if residual is None else residual.detach(), False)
+    return q if residual is None else (q, t)
 
 
 class _RmsNormLinear(torch.autograd.Function):
-    """Norm, quantisation and product in two launches (three with the weight's quantisation); the normalised rows exist
-    only as codes.  The backward pass recomputes them from the stored sum, straight into the column blocks that the weight
-    gradient wants, and keeps the gradient of the normalised rows in fp32 between the product and the norm."""
+    """The normalised rows exist only as codes.  The backward pass recomputes them from the stored sum, in the column blocks
+    that the weight gradient wants, and keeps the gradient of the normalised rows in fp32 between the product and the norm.
+    (CUDA calls take the native form of the same function.)"""
 
     @staticmethod
     def forward(ctx: Any, x: torch.Tensor, gain: torch.Tensor | None, w: torch.Tensor, b: torch.Tensor | None, eps: float,
@@ -250,15 +206,26 @@ def rms_norm_linear(x: torch.Tensor, norm_weight: torch.Tensor | None, weight: "
         w = weight.dequantize() if prepared else weight.float()
         y = torch.nn.functional.linear(h.float(), w, None if bias is None else bias.float()).to(out_dtype)
         return y if residual is None else (y, t)
-    x2, r2 = _rows(x, K), _rows(residual, K)
-    if x2.dim() == 1:
-        x2, r2 = x2[None], None if r2 is None else r2[None]
     if prepared:
-        q, t, _ = _norm_to_codes(x2.detach(), norm_weight, eps, None if r2 is None else r2.detach(), False)
-        y = _product(q, weight, None if bias is None else bias.detach(), out_dtype)
-    else:
-        gx, gn, gw, gr = _grads(x, norm_weight, weight, residual)
-        out = _RmsNormLinear.apply(x2, norm_weight, weight, bias, eps, r2, out_dtype, gx or gn or gr, gw)
-        y, t = (out, None) if residual is None else out
-    y = y.view(*x.shape[:-1], N)
-    return y if residual is None else (y, t.view(x.shape))
+        x, b, r = x.detach(), None if bias is None else bias.detach(), None if residual is None else residual.detach()
+        out = None
+        if x.is_cuda:
+            from ...ops import scaled_fused
+
+            out = scaled_fused.maybe_prepared_norm_linear(x, norm_weight, weight, b, r, eps, out_dtype)
+        if out is None:
+            q, t, _ = _norm_to_codes(x, norm_weight, eps, r, False)
+            out = _product(q, weight, b, out_dtype), t
+        return out[0] if residual is None else out
+    gx, gn, gw, gr = _grads(x, norm_weight, weight, residual)
+    if x.is_cuda:
+        from ...ops import scaled_fused
+
+        out = scaled_fused.maybe_fused_rms_norm_linear(x, norm_weight, weight, bias, residual, eps, out_dtype, gx or gn or gr, gw)
+        if out is not None:
+            return out[0] if residual is None else out
+    out = _RmsNormLinear.apply(x.reshape(M, K), norm_weight, weight, bias, eps, None if residual is None else residual.reshape(M, K),
+                               out_dtype, gx or gn or gr, gw)
+    if residual is None:
+        return out.view(*x.shape[:-1], N)
+    return out[0].view(*x.shape[:-1], N), out[1].view(x.shape)

@@ -2,21 +2,29 @@
 
 The library is a plain C-ABI shared object (``libjb_kernels.so``) next to this file, loaded
 with :mod:`ctypes`.  It is compiled for ``sm_100a`` only; nvcc cross-compiles on a machine
-without a GPU.
+without a GPU.  Beside it stands a torch binding (``_jb_torch.so``, host code only, compiled with the
+C++ compiler against torch's headers) that drives the 8-bit kernels without Python between the launches.
 """
 
 from __future__ import annotations
 
 import hashlib
+import importlib.machinery
+import importlib.util
 import os
 import shutil
 import subprocess
+import sysconfig
 from pathlib import Path
+from typing import Any
 
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB_PATH = HERE / "libjb_kernels.so"
 _STAMP = HERE / "libjb_kernels.stamp"
+BINDING_PATH = HERE / "_jb_torch.so"
+_BINDING_STAMP = HERE / "_jb_torch.stamp"
+_BINDING_SOURCES = ("torch_binding.cpp", "scaled_abi.h")
 
 NVCC_FLAGS = [
     "-gencode",
@@ -72,7 +80,61 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return LIB_PATH
 
 
+# ----------------------------------------------------------------------------- torch binding
+def _cuda_home() -> Path:
+    nvcc = _nvcc()
+    return Path(nvcc).resolve().parent.parent if nvcc else Path("/usr/local/cuda")
+
+
+def binding_hash() -> str:
+    import torch
+
+    h = hashlib.sha256()
+    for name in _BINDING_SOURCES:
+        h.update((CSRC / name).read_bytes())
+    h.update(f"{torch.__version__} {sysconfig.get_python_version()}".encode())
+    return h.hexdigest()
+
+
+def binding_is_fresh() -> bool:
+    return BINDING_PATH.exists() and _BINDING_STAMP.exists() and _BINDING_STAMP.read_text().strip() == binding_hash()
+
+
+def build_binding(force: bool = False) -> Path:
+    """Compile ``csrc/torch_binding.cpp`` into ``_jb_torch.so`` if it or torch changed."""
+    if not force and binding_is_fresh():
+        return BINDING_PATH
+    import torch
+
+    cxx = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("no C++ compiler found; cannot build the torch binding of jigsaw_b200")
+    root = Path(torch.__file__).parent
+    tmp = BINDING_PATH.with_suffix(".so.tmp%d" % os.getpid())
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}", f"-I{_cuda_home() / 'include'}",
+           f"-I{sysconfig.get_paths()['include']}", str(CSRC / "torch_binding.cpp"), "-o", str(tmp), f"-L{root / 'lib'}",
+           "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10", "-lc10_cuda"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError("the C++ compiler failed on the torch binding:\n" + proc.stdout + proc.stderr)
+    os.replace(tmp, BINDING_PATH)
+    _BINDING_STAMP.write_text(binding_hash())
+    return BINDING_PATH
+
+
+def load_binding() -> Any:
+    """The extension module, built first if its source is newer."""
+    path = str(build_binding())
+    loader = importlib.machinery.ExtensionFileLoader("_jb_torch", path)
+    spec = importlib.util.spec_from_file_location("_jb_torch", path, loader=loader)
+    module = importlib.util.module_from_spec(spec)
+    loader.exec_module(module)
+    return module
+
+
 if __name__ == "__main__":
     import sys
 
     print(build(force="--force" in sys.argv, verbose="-v" in sys.argv))
+    print(build_binding(force="--force" in sys.argv))

@@ -12,6 +12,7 @@ import ctypes
 import os
 from ctypes import POINTER, c_int, c_longlong, c_uint, c_void_p, c_float
 from functools import lru_cache
+from typing import Any
 
 import torch
 
@@ -94,58 +95,9 @@ class JbAdamTensors(ctypes.Structure):
                 ("numel", c_longlong * 48), ("count", c_int)]
 
 
-class JbScaledOperand(ctypes.Structure):
-    """One operand of the 8-bit matrix product (see ``csrc/scaled_gemm.cu``)."""
-
-    _fields_ = [("codes", c_void_p), ("pitch", c_longlong), ("scales", c_void_p), ("scale_row", c_longlong),
-                ("scale_k", c_longlong), ("rows", c_int), ("square", c_int)]
-
-
-class JbQuant(ctypes.Structure):
-    """Arguments of the block quantisation (see ``csrc/scaled_quant.cu``)."""
-
-    _fields_ = [("x", c_void_p), ("ldx", c_longlong), ("rows", c_int), ("cols", c_int), ("type", c_int), ("square", c_int),
-                ("codes", c_void_p), ("pitch", c_longlong), ("scales", c_void_p), ("scale_row", c_longlong),
-                ("scale_k", c_longlong), ("codes_t", c_void_p), ("pitch_t", c_longlong), ("scales_t", c_void_p),
-                ("scale_t_row", c_longlong), ("scale_t_k", c_longlong), ("rstd", c_void_p), ("gain", c_void_p),
-                ("gain_type", c_int), ("colsum", c_void_p)]
-
-
-class JbRms(ctypes.Structure):
-    """Arguments of the forward root-mean-square norm (see ``csrc/scaled_quant.cu``)."""
-
-    _fields_ = [("x", c_void_p), ("residual", c_void_p), ("ldx", c_longlong), ("ldr", c_longlong), ("rows", c_int),
-                ("cols", c_int), ("type", c_int), ("eps", c_float), ("gain", c_void_p), ("gain_type", c_int), ("sum", c_void_p),
-                ("rstd", c_void_p), ("y", c_void_p), ("y_type", c_int), ("codes", c_void_p), ("pitch", c_longlong),
-                ("scales", c_void_p), ("scale_row", c_longlong), ("scale_k", c_longlong)]
-
-
-class JbRmsBwd(ctypes.Structure):
-    """Arguments of the backward root-mean-square norm (see ``csrc/scaled_quant.cu``)."""
-
-    _fields_ = [("t", c_void_p), ("ldt", c_longlong), ("g", c_void_p), ("g_f32", c_int), ("gsum", c_void_p), ("rstd", c_void_p),
-                ("gain", c_void_p), ("gain_type", c_int), ("rows", c_int), ("cols", c_int), ("type", c_int), ("dx", c_void_p),
-                ("part", c_void_p)]
-
-
 def _declare(L: ctypes.CDLL) -> None:
-    L.jb_scaled_gemm.argtypes = [POINTER(JbScaledOperand), POINTER(JbScaledOperand), c_longlong, c_void_p, c_longlong, c_int,
-                                 c_void_p, c_int, c_int, c_void_p, c_void_p]
-    L.jb_scaled_gemm.restype = c_int
-    L.jb_quantize.argtypes = [POINTER(JbQuant), c_void_p]
-    L.jb_quantize.restype = c_int
-    L.jb_column_sum.argtypes = [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]
-    L.jb_column_sum.restype = c_int
     L.jb_rms_max_cols.argtypes = []
     L.jb_rms_max_cols.restype = c_int
-    L.jb_rms_norm_fwd.argtypes = [POINTER(JbRms), c_void_p]
-    L.jb_rms_norm_fwd.restype = c_int
-    L.jb_rms_bwd_grid.argtypes = [c_int, c_int, c_int]
-    L.jb_rms_bwd_grid.restype = c_int
-    L.jb_rms_bwd_parts.argtypes = [c_int, c_int, c_int]
-    L.jb_rms_bwd_parts.restype = c_int
-    L.jb_rms_norm_bwd.argtypes = [POINTER(JbRmsBwd), c_int, c_void_p]
-    L.jb_rms_norm_bwd.restype = c_int
     L.jb_abi_version.restype = c_int
     L.jb_gemm_bf16.argtypes = [
         c_void_p, c_void_p, c_void_p, c_void_p,  # A B C bias
@@ -340,13 +292,26 @@ def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
-#: Number of kernels of this library launched so far in this process (benchmarks report it).
-LAUNCHES = 0
+# ``LAUNCHES``: number of kernels of this library launched so far in this process (benchmarks report it), the sum of the
+# launches counted here and by the native binding.
+_launches = 0
+_launch_counters: list = []
 
 
 def count_launches(n: int = 1) -> None:
-    global LAUNCHES
-    LAUNCHES += n
+    global _launches
+    _launches += n
+
+
+def add_launch_counter(read: Any) -> None:
+    """``read()`` returns the launches that some other part of the process made."""
+    _launch_counters.append(read)
+
+
+def __getattr__(name: str) -> int:
+    if name == "LAUNCHES":
+        return _launches + sum(read() for read in _launch_counters)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 # ----------------------------------------------------------------------------- audited dispatch

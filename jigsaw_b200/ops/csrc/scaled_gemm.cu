@@ -15,6 +15,7 @@
 #include <type_traits>
 
 #include "ptx.cuh"
+#include "scaled_abi.h"
 #include "tmap.cuh"
 
 namespace jb {
@@ -506,17 +507,6 @@ static int launch_scaled_gemm(const void* P, long long pitch_p, const void* Q, l
 }
 
 }  // namespace jb
-
-// One operand of jb_scaled_gemm: e4m3 codes [rows, K] (K contiguous, rows `pitch` bytes apart, base and pitch multiples
-// of 16) and their e8m0 scales, strides in bytes per scale row and per block of 128 along K.
-struct JbScaledOperand {
-  const void* codes;
-  long long pitch;
-  const void* scales;
-  long long scale_row, scale_k;
-  int rows;
-  int square;                  // 0: a scale per row, 1: per 128 rows
-};
 
 extern "C" int jb_scaled_gemm(const JbScaledOperand* a, const JbScaledOperand* b, long long K, void* out, long long ldo,
                               int out_type, const void* bias, int bias_type, int sm_count, int* status, void* stream) {

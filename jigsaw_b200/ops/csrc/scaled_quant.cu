@@ -10,6 +10,7 @@
 #include <cuda_fp8.h>
 
 #include "ptx.cuh"
+#include "scaled_abi.h"
 
 namespace jb {
 
@@ -573,25 +574,6 @@ static int launch_quant(const QuantArgs& a, bool tiles, cudaStream_t st) {
 
 }  // namespace jb
 
-// Element types of this file's entry points: 0 fp32, 1 bf16, 2 fp16.
-struct JbQuant {
-  const void* x;
-  long long ldx;
-  int rows, cols, type, square;
-  void* codes;
-  long long pitch;
-  void* scales;
-  long long scale_row, scale_k;
-  void* codes_t;
-  long long pitch_t;
-  void* scales_t;
-  long long scale_t_row, scale_t_k;
-  const void* rstd;
-  const void* gain;
-  int gain_type;
-  void* colsum;
-};
-
 // Codes and scales of x (times rstd and gain) by rows, by columns (transposed), both, or in squares of 128 x 128 (both
 // layouts share the scales).  Pitches are multiples of 16; bytes between the last value and the pitch are written as 0
 // within the last 8 (transposed: 16) bytes only.
@@ -622,24 +604,6 @@ extern "C" int jb_column_sum(const float* part, int P, int C, void* out, int out
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
-struct JbRms {
-  const void* x;
-  const void* residual;
-  long long ldx, ldr;
-  int rows, cols, type;
-  float eps;
-  const void* gain;
-  int gain_type;
-  void* sum;
-  void* rstd;
-  void* y;
-  int y_type;                // the type of x, or 0
-  void* codes;
-  long long pitch;
-  void* scales;
-  long long scale_row, scale_k;
-};
-
 // Longest row that the kernels keep in registers.
 extern "C" int jb_rms_max_cols() { return 32768; }
 
@@ -663,20 +627,6 @@ extern "C" int jb_rms_norm_fwd(const JbRms* q, void* stream) {
   if (q->type == 2) return vec ? launch_rms_fwd<__half, true>(a, st) : launch_rms_fwd<__half, false>(a, st);
   return -1;
 }
-
-struct JbRmsBwd {
-  const void* t;
-  long long ldt;
-  const void* g;
-  int g_f32;
-  const void* gsum;
-  const void* rstd;
-  const void* gain;
-  int gain_type;
-  int rows, cols, type;
-  void* dx;
-  void* part;
-};
 
 // CTAs of the backward pass and rows of its partial sums.  Two CTAs an SM fill it; a CTA takes at least four rounds of
 // rows, so that the partial sums stay a small part of the traffic.

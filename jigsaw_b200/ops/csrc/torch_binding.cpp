@@ -1,0 +1,619 @@
+// Torch binding of the 8-bit kernels: buffers, launches and backward passes without Python between them.
+//
+// A training step of one 8-bit linear layer is seven launches and about sixteen buffers; driven from Python it costs
+// several times what the kernels take on a short batch (measured on 1021 x 1000 x 2056: 350 us of host time against
+// 40 us of kernels).  The functions here allocate with torch's allocator on every call and keep nothing between calls.
+// The kernel library is loaded by Python, which hands its entry points over in init(): the binding links against torch
+// only.
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <atomic>
+#include <optional>
+
+#include "scaled_abi.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+
+struct Api {
+  decltype(&jb_scaled_gemm) gemm = nullptr;
+  decltype(&jb_quantize) quantize = nullptr;
+  decltype(&jb_column_sum) column_sum = nullptr;
+  decltype(&jb_rms_norm_fwd) rms_fwd = nullptr;
+  decltype(&jb_rms_bwd_parts) rms_bwd_parts = nullptr;
+  decltype(&jb_rms_norm_bwd) rms_bwd = nullptr;
+} api;
+
+std::atomic<long long> launches{0};
+
+constexpr auto CODES = at::kFloat8_e4m3fn;
+constexpr auto SCALES = at::kFloat8_e8m0fnu;
+
+int type_of(at::ScalarType t) {
+  if (t == at::kFloat) return 0;
+  if (t == at::kBFloat16) return 1;
+  TORCH_CHECK_TYPE(t == at::kHalf, "the 8-bit kernels take fp32, bf16 and fp16, got ", t);
+  return 2;
+}
+at::ScalarType scalar_of(int64_t type) { return type == 0 ? at::kFloat : type == 1 ? at::kBFloat16 : at::kHalf; }
+
+void done(int rc, const char* what, int n = 1) {
+  TORCH_CHECK(rc == 0, "jigsaw_b200 kernel launcher ", what, " failed with code ", rc);
+  launches.fetch_add(n, std::memory_order_relaxed);
+}
+
+Tensor empty(at::IntArrayRef sizes, at::ScalarType t, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, t, like.device(), std::nullopt);
+}
+void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+int sm_count(const Tensor& t) { return at::cuda::getDeviceProperties(t.device().index())->multiProcessorCount; }
+int checked(int64_t n) {
+  TORCH_CHECK_VALUE(n <= 0x7fffff00LL, "an axis of ", n, " elements is longer than the kernels address");
+  return static_cast<int>(n);
+}
+int64_t pitch_of(int64_t n) { return (n + 15) / 16 * 16; }
+
+// A tensor as rows of its last axis, `ld` elements apart; copied only if its strides do not allow that.
+struct Rows {
+  Tensor t;
+  int64_t rows, cols, ld;
+};
+Rows rows_of(const Tensor& x) {
+  const int64_t c = x.size(-1), r = x.numel() / c;
+  if (x.is_contiguous()) return {x, r, c, c};
+  if (x.dim() == 2 && (x.stride(1) == 1 || c == 1) && x.stride(0) >= 0) return {x, r, c, x.stride(0)};
+  return {x.contiguous(), r, c, c};
+}
+
+// Codes [rows, pitch] and scales of a quantised matrix.
+struct Codes {
+  Tensor codes, scales;
+  int64_t rows = 0, cols = 0, scale_row = 0, scale_k = 0;
+  bool square = false;
+  bool turned = false;       // `scales` is stored blocks first
+
+  JbScaledOperand operand() const {
+    return {codes.data_ptr(), codes.size(1), scales.data_ptr(), scale_row, scale_k, static_cast<int>(rows), square ? 1 : 0};
+  }
+  // The public forms: [rows, cols] and [scale rows, blocks].
+  Tensor code_view() const { return codes.size(1) == cols ? codes : codes.narrow(1, 0, cols); }
+  Tensor scale_view() const { return turned ? scales.t() : scales; }
+};
+// Scales per row are stored block by block, rows contiguous: a warp of the product reads 32 rows in one request.
+Codes new_codes(int64_t rows, int64_t cols, const Tensor& like) {
+  Codes q;
+  q.rows = rows;
+  q.cols = cols;
+  q.codes = empty({rows, pitch_of(cols)}, CODES, like);
+  return q;
+}
+void new_row_scales(Codes& q) {
+  q.scales = empty({(q.cols + 127) / 128, q.rows}, SCALES, q.codes);
+  q.scale_row = 1;
+  q.scale_k = q.rows;
+  q.turned = true;
+}
+
+struct Quantized {
+  std::optional<Codes> rows, cols;
+  Tensor sums;
+};
+
+// Codes of x (of x * rstd * gain) along its rows and / or of its transpose along the columns, read once; `sum_type` >= 0
+// asks for the column sums.
+Quantized quantize(const Tensor& input, bool square, bool want_rows, bool want_cols, const Tensor& rstd, const Tensor& gain,
+                   int sum_type) {
+  const c10::cuda::CUDAGuard guard(input.device());
+  const Rows x = rows_of(input);
+  const int64_t rb = (x.rows + 127) / 128, cb = (x.cols + 127) / 128;
+  JbQuant q{};
+  q.x = x.t.const_data_ptr();
+  q.ldx = x.ld;
+  q.rows = checked(x.rows);
+  q.cols = checked(x.cols);
+  q.type = type_of(x.t.scalar_type());
+  q.square = square;
+  Quantized out;
+  Tensor shared;
+  if (square) {
+    shared = empty({rb, cb}, SCALES, x.t);
+    q.scales = shared.data_ptr();
+    q.scale_row = cb;
+    q.scale_k = 1;
+  }
+  if (want_rows) {
+    Codes c = new_codes(x.rows, x.cols, x.t);
+    q.codes = c.codes.data_ptr();
+    q.pitch = c.codes.size(1);
+    if (square) {
+      c.scales = shared;
+      c.scale_row = cb;
+      c.scale_k = 1;
+      c.square = true;
+    } else {
+      new_row_scales(c);
+      q.scales = c.scales.data_ptr();
+      q.scale_row = c.scale_row;
+      q.scale_k = c.scale_k;
+    }
+    out.rows = std::move(c);
+  }
+  if (want_cols) {
+    Codes c = new_codes(x.cols, x.rows, x.t);
+    q.codes_t = c.codes.data_ptr();
+    q.pitch_t = c.codes.size(1);
+    if (square) {
+      c.scales = shared;
+      c.scale_row = 1;
+      c.scale_k = cb;
+      c.square = c.turned = true;
+    } else {
+      new_row_scales(c);
+      q.scales_t = c.scales.data_ptr();
+      q.scale_t_row = c.scale_row;
+      q.scale_t_k = c.scale_k;
+    }
+    out.cols = std::move(c);
+  }
+  Tensor gain_c;
+  if (rstd.defined()) {
+    q.rstd = rstd.const_data_ptr();
+    if (gain.defined()) {
+      gain_c = gain.contiguous();
+      q.gain = gain_c.const_data_ptr();
+      q.gain_type = type_of(gain_c.scalar_type());
+    }
+  }
+  Tensor part;
+  if (sum_type >= 0) {
+    part = empty({rb, x.cols}, at::kFloat, x.t);
+    q.colsum = part.data_ptr();
+  }
+  done(api.quantize(&q, stream_of(x.t)), "quantize");
+  if (sum_type >= 0) {
+    out.sums = empty({x.cols}, scalar_of(sum_type), x.t);
+    done(api.column_sum(part.const_data_ptr<float>(), checked(rb), q.cols, out.sums.data_ptr(), sum_type, stream_of(x.t)), "column_sum");
+  }
+  return out;
+}
+
+// a [M, K] b [N, K]^T + bias, as a tensor of the given sizes (M N elements).
+Tensor product(const JbScaledOperand& a, const JbScaledOperand& b, int64_t K, const Tensor& bias, int out_type,
+               at::IntArrayRef sizes, const Tensor& like, const Tensor& status) {
+  Tensor out = empty(sizes, scalar_of(out_type), like);
+  Tensor bias_c;
+  if (bias.defined()) bias_c = bias.contiguous();
+  done(api.gemm(&a, &b, K, out.data_ptr(), b.rows, out_type, bias.defined() ? bias_c.const_data_ptr() : nullptr,
+                bias.defined() ? type_of(bias_c.scalar_type()) : 0, sm_count(like), status.data_ptr<int>(), stream_of(like)),
+       "scaled_gemm");
+  return out;
+}
+
+struct Normed {
+  Tensor y, sum, rstd;
+  std::optional<Codes> codes;
+};
+
+Normed rms_forward(const Tensor& input, const Tensor& gain, double eps, const Tensor& residual, int y_type, bool want_codes,
+                   bool want_rstd) {
+  const c10::cuda::CUDAGuard guard(input.device());
+  const Rows x = rows_of(input);
+  JbRms q{};
+  q.x = x.t.const_data_ptr();
+  q.ldx = x.ld;
+  q.rows = checked(x.rows);
+  q.cols = checked(x.cols);
+  q.type = type_of(x.t.scalar_type());
+  q.eps = static_cast<float>(eps);
+  Tensor gain_c;
+  if (gain.defined()) {
+    gain_c = gain.contiguous();
+    q.gain = gain_c.const_data_ptr();
+    q.gain_type = type_of(gain_c.scalar_type());
+  }
+  Normed out;
+  Rows r;
+  if (residual.defined()) {
+    r = rows_of(residual);
+    q.residual = r.t.const_data_ptr();
+    q.ldr = r.ld;
+    out.sum = empty(input.sizes(), x.t.scalar_type(), x.t);
+    q.sum = out.sum.data_ptr();
+  }
+  if (want_rstd) {
+    out.rstd = empty({x.rows}, at::kFloat, x.t);
+    q.rstd = out.rstd.data_ptr();
+  }
+  if (y_type >= 0) {
+    out.y = empty(input.sizes(), scalar_of(y_type), x.t);
+    q.y = out.y.data_ptr();
+    q.y_type = y_type;
+  }
+  if (want_codes) {
+    Codes c = new_codes(x.rows, x.cols, x.t);
+    new_row_scales(c);
+    q.codes = c.codes.data_ptr();
+    q.pitch = c.codes.size(1);
+    q.scales = c.scales.data_ptr();
+    q.scale_row = c.scale_row;
+    q.scale_k = c.scale_k;
+    out.codes = std::move(c);
+  }
+  done(api.rms_fwd(&q, stream_of(x.t)), "rms_norm_fwd");
+  return out;
+}
+
+// Gradients of the normalised sum t and of the gain; g has the type of t or fp32.
+std::pair<Tensor, Tensor> rms_backward(const Tensor& sum, const Tensor& gain, const Tensor& rstd, const Tensor& grad,
+                                       const Tensor& grad_sum, bool want_gain) {
+  const c10::cuda::CUDAGuard guard(sum.device());
+  const Rows t = rows_of(sum);
+  Tensor g = grad, gs = grad_sum, gain_c;
+  if (g.scalar_type() != sum.scalar_type() && g.scalar_type() != at::kFloat) g = g.to(at::kFloat);
+  g = g.contiguous();
+  JbRmsBwd q{};
+  q.t = t.t.const_data_ptr();
+  q.ldt = t.ld;
+  q.rows = checked(t.rows);
+  q.cols = checked(t.cols);
+  q.type = type_of(t.t.scalar_type());
+  q.g = g.const_data_ptr();
+  q.g_f32 = g.scalar_type() == at::kFloat;
+  if (gs.defined()) {
+    gs = gs.to(sum.scalar_type()).contiguous();
+    q.gsum = gs.const_data_ptr();
+  }
+  q.rstd = rstd.const_data_ptr();
+  if (gain.defined()) {
+    gain_c = gain.contiguous();
+    q.gain = gain_c.const_data_ptr();
+    q.gain_type = type_of(gain_c.scalar_type());
+  }
+  Tensor dx = empty(sum.sizes(), sum.scalar_type(), sum), dgain, part;
+  q.dx = dx.data_ptr();
+  const int sm = sm_count(sum);
+  if (want_gain) {
+    part = empty({api.rms_bwd_parts(q.rows, q.cols, sm), t.cols}, at::kFloat, sum);
+    q.part = part.data_ptr();
+  }
+  done(api.rms_bwd(&q, sm, stream_of(sum)), "rms_norm_bwd");
+  if (want_gain) {
+    dgain = empty({t.cols}, gain.scalar_type(), sum);
+    done(api.column_sum(part.const_data_ptr<float>(), checked(part.size(0)), q.cols, dgain.data_ptr(), q.gain_type, stream_of(sum)),
+         "column_sum");
+  }
+  return {dx, dgain};
+}
+
+// ------------------------------------------------------------------------------------------------ autograd
+using Optional = std::optional<Tensor>;
+Tensor opt(const Optional& t) { return t.has_value() ? *t : Tensor(); }
+
+// The backward passes are kernels without a derivative of their own: with create_graph=True the gradients carry a node
+// that raises when it is differentiated.
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list real;
+  for (auto& g : grads)
+    if (g.defined()) real.push_back(g.detach().requires_grad_(true));
+  if (real.empty()) return grads;
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      "trying to differentiate twice a function that is differentiable once (8-bit path)", static_cast<int64_t>(real.size()));
+  variable_list marked = (*error)(std::move(real));
+  size_t k = 0;
+  for (auto& g : grads)
+    if (g.defined()) g = marked[k++];
+  return grads;
+}
+
+void save_codes(variable_list& to, const std::optional<Codes>& c) {
+  to.push_back(c ? c->codes : Tensor());
+  to.push_back(c ? c->scales : Tensor());
+}
+// The transposed weight, or the activations in blocks along the tokens, as saved by the forward pass.
+Codes saved_codes(const Tensor& codes, const Tensor& scales, int64_t rows, int64_t cols, bool square) {
+  Codes c;
+  c.codes = codes;
+  c.scales = scales;
+  c.rows = rows;
+  c.cols = cols;
+  c.square = square;
+  c.scale_row = 1;
+  c.scale_k = scales.size(1);
+  return c;
+}
+std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
+  std::vector<int64_t> s = x.sizes().vec();
+  s.back() = n;
+  return s;
+}
+
+struct LinearGrads {
+  Tensor dx, dw, db;
+};
+// The two gradient products of a layer whose transposed weight and column-quantised input are given (absent: not wanted).
+LinearGrads linear_backward(const Tensor& g, const std::optional<Codes>& w_t, const std::optional<Codes>& x_t, int dx_type,
+                            at::IntArrayRef dx_sizes, int dw_type, int bias_type, const Tensor& status) {
+  LinearGrads out;
+  const Quantized q = quantize(g, false, w_t.has_value(), x_t.has_value(), Tensor(), Tensor(), bias_type);
+  const int64_t N = g.size(-1), M = g.numel() / N;
+  if (w_t) out.dx = product(q.rows->operand(), w_t->operand(), N, Tensor(), dx_type, dx_sizes, g, status);
+  if (x_t) out.dw = product(q.cols->operand(), x_t->operand(), M, Tensor(), dw_type, {N, x_t->rows}, g, status);
+  out.db = q.sums;
+  return out;
+}
+Tensor bias_sum(const Tensor& g, int type) {
+  return at::sum(g.reshape({-1, g.size(-1)}), {0}, false, at::kFloat).to(scalar_of(type));
+}
+
+// y = q(x) q(w)^T + b; dx = q(g) q(w); dw = q(g^T) q(x^T)^T with blocks along the tokens.  x and w are read once and
+// written in the layouts that all three products want.
+struct ScaledLinear : public Function<ScaledLinear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Optional& bias, int64_t out_type, bool need_x,
+                        bool need_w, const Tensor& status) {
+    const Tensor b = opt(bias);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Quantized qx = quantize(x, false, true, need_w, Tensor(), Tensor(), -1);
+    const Quantized qw = quantize(w, true, true, need_x, Tensor(), Tensor(), -1);
+    variable_list save;
+    save_codes(save, qx.cols);
+    save_codes(save, qw.cols);
+    save.push_back(status);
+    ctx->save_for_backward(save);
+    ctx->saved_data["x"] = x.sizes().vec();
+    ctx->saved_data["n"] = w.size(0);
+    ctx->saved_data["types"] = std::vector<int64_t>{type_of(x.scalar_type()), type_of(w.scalar_type()),
+                                                    b.defined() ? type_of(b.scalar_type()) : -1};
+    ctx->set_materialize_grads(false);
+    return product(qx.rows->operand(), qw.rows->operand(), x.size(-1), b, static_cast<int>(out_type), with_last(x, w.size(0)), x, status);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(7);
+    const Tensor g = grads[0];
+    if (!g.defined()) return out;
+    const c10::cuda::CUDAGuard guard(g.device());
+    const variable_list s = ctx->get_saved_variables();
+    const std::vector<int64_t> xs = ctx->saved_data["x"].toIntVector(), types = ctx->saved_data["types"].toIntVector();
+    const int64_t N = ctx->saved_data["n"].toInt(), K = xs.back();
+    int64_t M = 1;
+    for (size_t i = 0; i + 1 < xs.size(); ++i) M *= xs[i];
+    std::optional<Codes> x_t, w_t;
+    if (s[0].defined() && ctx->needs_input_grad(1)) x_t = saved_codes(s[0], s[1], K, M, false);
+    if (s[2].defined() && ctx->needs_input_grad(0)) w_t = saved_codes(s[2], s[3], K, N, true);
+    const int bias_type = types[2] >= 0 && ctx->needs_input_grad(2) ? static_cast<int>(types[2]) : -1;
+    if (x_t || w_t) {
+      LinearGrads l = linear_backward(g, w_t, x_t, static_cast<int>(types[0]), xs, static_cast<int>(types[1]), bias_type, s[4]);
+      out[0] = l.dx;
+      out[1] = l.dw;
+      out[2] = l.db;
+    } else if (bias_type >= 0) {
+      out[2] = bias_sum(g, bias_type);
+    }
+    return once(std::move(out));
+  }
+};
+
+// y = t r gain, t = x + residual; outputs (y, t), or y alone.
+struct RmsNorm : public Function<RmsNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Optional& gain_in, const Optional& residual_in, double eps,
+                               int64_t y_type, bool need) {
+    const Tensor gain = opt(gain_in), residual = opt(residual_in);
+    Normed n = rms_forward(x, gain, eps, residual, static_cast<int>(y_type), false, need);
+    ctx->set_materialize_grads(false);
+    if (need) ctx->save_for_backward({residual.defined() ? n.sum : x, gain, n.rstd});
+    ctx->saved_data["residual"] = residual.defined();
+    return residual.defined() ? variable_list{n.y, n.sum} : variable_list{n.y};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(6);
+    const variable_list s = ctx->get_saved_variables();
+    const bool residual = ctx->saved_data["residual"].toBool();
+    const Tensor gsum = residual ? grads[1] : Tensor();
+    const bool want_gain = s[1].defined() && ctx->needs_input_grad(1);
+    if (grads[0].defined()) {
+      std::tie(out[0], out[1]) = rms_backward(s[0], s[1], s[2], grads[0], gsum, want_gain);
+    } else {                                   // only the sum was used
+      if (gsum.defined()) out[0] = gsum.to(s[0].scalar_type());
+      if (want_gain) out[1] = at::zeros_like(s[1]);
+    }
+    if (residual) out[2] = out[0];
+    return once(std::move(out));
+  }
+};
+
+// The norm's output exists as codes only; the backward pass normalises the stored sum again, straight into the column
+// blocks of the weight gradient, and keeps the gradient of the normalised rows in fp32 between product and norm.
+struct RmsNormLinear : public Function<RmsNormLinear> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Optional& gain_in, const Tensor& w, const Optional& bias,
+                               const Optional& residual_in, double eps, int64_t out_type, bool need_h, bool need_w,
+                               const Tensor& status) {
+    const Tensor gain = opt(gain_in), b = opt(bias), residual = opt(residual_in);
+    const c10::cuda::CUDAGuard guard(x.device());
+    Normed n = rms_forward(x, gain, eps, residual, -1, true, need_h || need_w);
+    const Quantized qw = quantize(w, true, true, need_h, Tensor(), Tensor(), -1);
+    ctx->set_materialize_grads(false);
+    variable_list save;
+    if (need_h || need_w) {
+      save = {residual.defined() ? n.sum : x, gain, n.rstd};
+      save_codes(save, qw.cols);
+      save.push_back(status);
+    }
+    ctx->save_for_backward(save);
+    ctx->saved_data["flags"] = std::vector<int64_t>{need_h, need_w, residual.defined(), w.size(0), type_of(w.scalar_type()),
+                                                    b.defined() ? type_of(b.scalar_type()) : -1, gain.defined()};
+    Tensor y = product(n.codes->operand(), qw.rows->operand(), x.size(-1), b, static_cast<int>(out_type), with_last(x, w.size(0)), x, status);
+    return residual.defined() ? variable_list{y, n.sum} : variable_list{y};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(10);
+    const std::vector<int64_t> f = ctx->saved_data["flags"].toIntVector();
+    const bool need_h = f[0], need_w = f[1], residual = f[2];
+    const int64_t N = f[3];
+    const Tensor g = grads[0], gsum = residual ? grads[1] : Tensor();
+    // edges count the tensors that were given: x, [gain], w, [bias], [residual]
+    const size_t w_edge = f[6] ? 2 : 1, residual_edge = w_edge + (f[5] >= 0 ? 2 : 1);
+    const int bias_type = f[5] >= 0 && ctx->needs_input_grad(w_edge + 1) ? static_cast<int>(f[5]) : -1;
+    const variable_list s = ctx->get_saved_variables();
+    if (!need_h && !need_w) {
+      if (g.defined() && bias_type >= 0) out[3] = bias_sum(g, bias_type);
+      return once(std::move(out));
+    }
+    const Tensor &t = s[0], &gain = s[1], &rstd = s[2];
+    const c10::cuda::CUDAGuard guard(t.device());
+    const int64_t K = t.size(-1);
+    const bool want_gain = gain.defined() && ctx->needs_input_grad(1);
+    const bool want_h = need_h && (want_gain || ctx->needs_input_grad(0) || (residual && ctx->needs_input_grad(residual_edge)));
+    Tensor dh;
+    if (g.defined()) {
+      std::optional<Codes> w_t, h_t;
+      if (want_h) w_t = saved_codes(s[3], s[4], K, N, true);
+      if (need_w && ctx->needs_input_grad(w_edge)) h_t = quantize(t, false, false, true, rstd, gain, -1).cols;
+      if (w_t || h_t) {
+        LinearGrads l = linear_backward(g, w_t, h_t, 0, t.sizes(), static_cast<int>(f[4]), bias_type, s[5]);
+        dh = l.dx;
+        out[2] = l.dw;
+        out[3] = l.db;
+      } else if (bias_type >= 0) {
+        out[3] = bias_sum(g, bias_type);
+      }
+    }
+    if (dh.defined()) {
+      std::tie(out[0], out[1]) = rms_backward(t, gain, rstd, dh, gsum, want_gain);
+    } else {
+      if (gsum.defined()) out[0] = gsum.to(t.scalar_type());
+      if (want_gain) out[1] = at::zeros_like(gain);
+    }
+    if (residual) out[4] = out[0];
+    return once(std::move(out));
+  }
+};
+
+// ------------------------------------------------------------------------------------------------ Python
+py::object give(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
+
+py::tuple py_quantize(const Tensor& x, bool square, bool rows, bool cols, const Optional& rstd,
+                      const Optional& gain, int sum_type) {
+  const Quantized q = quantize(x, square, rows, cols, opt(rstd), opt(gain), sum_type);
+  return py::make_tuple(q.rows ? give(q.rows->code_view()) : py::none(), q.rows ? give(q.rows->scale_view()) : py::none(),
+                        q.cols ? give(q.cols->code_view()) : py::none(), q.cols ? give(q.cols->scale_view()) : py::none(),
+                        give(q.sums));
+}
+
+// A public operand: codes that TMA cannot address (rows not on 16-byte boundaries, or not contiguous) are copied once.
+Codes operand_of(const Tensor& codes, const Tensor& scales, bool square) {
+  Codes c;
+  c.rows = codes.numel() / codes.size(-1);
+  c.cols = codes.size(-1);
+  checked(c.rows);
+  Tensor m = codes;
+  if (m.dim() != 2) m = m.reshape({c.rows, c.cols});
+  const int64_t pitch = c.rows > 1 ? m.stride(0) : pitch_of(c.cols);
+  if ((m.stride(1) != 1 && c.cols > 1) || pitch % 16 || pitch < c.cols || reinterpret_cast<uintptr_t>(m.const_data_ptr()) % 16) {
+    c.codes = empty({c.rows, pitch_of(c.cols)}, CODES, m);
+    c.codes.narrow(1, 0, c.cols).view(at::kByte).copy_(m.view(at::kByte));
+  } else {
+    // rows `pitch` bytes apart, as JbScaledOperand wants them; the view is never read through torch
+    c.codes = m;
+  }
+  c.scales = scales.dim() == 2 ? scales : scales.reshape({c.rows, scales.size(-1)});
+  c.scale_row = c.scales.stride(0);
+  c.scale_k = c.scales.stride(1);
+  c.square = square;
+  return c;
+}
+JbScaledOperand describe(const Codes& c) {
+  JbScaledOperand o = c.operand();
+  o.pitch = c.rows > 1 ? c.codes.stride(0) : pitch_of(c.cols);
+  return o;
+}
+
+Tensor py_scaled_matmul(const Tensor& a_codes, const Tensor& a_scales, bool a_square, const Tensor& b_codes, const Tensor& b_scales,
+                        bool b_square, const Optional& bias, int out_type, const Tensor& status) {
+  const c10::cuda::CUDAGuard guard(a_codes.device());
+  const Codes a = operand_of(a_codes, a_scales, a_square), b = operand_of(b_codes, b_scales, b_square);
+  return product(describe(a), describe(b), a.cols, opt(bias), out_type, with_last(a_codes, b.rows), a_codes, status);
+}
+
+py::tuple py_rms_quantize(const Tensor& x, const Optional& gain, double eps, const Optional& residual,
+                          bool want_rstd) {
+  const Normed n = rms_forward(x, opt(gain), eps, opt(residual), -1, true, want_rstd);
+  Tensor codes = n.codes->code_view(), scales = n.codes->scale_view();
+  if (x.dim() != 2) {
+    codes = codes.view(x.sizes());
+    scales = scales.view(with_last(x, scales.size(1)));
+  }
+  return py::make_tuple(give(codes), give(scales), give(n.sum), give(n.rstd));
+}
+
+// Inference forms with a prepared weight: quantisation (with or without the norm) and product, two launches.
+Tensor py_linear_prepared(const Tensor& x, const Tensor& w_codes, const Tensor& w_scales, bool w_square,
+                          const Optional& bias, int out_type, const Tensor& status) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Quantized q = quantize(x, false, true, false, Tensor(), Tensor(), -1);
+  const Codes w = operand_of(w_codes, w_scales, w_square);
+  return product(q.rows->operand(), describe(w), w.cols, opt(bias), out_type, with_last(x, w.rows), x, status);
+}
+py::tuple py_norm_linear_prepared(const Tensor& x, const Optional& gain, double eps, const Optional& residual,
+                                  const Tensor& w_codes, const Tensor& w_scales, bool w_square, const Optional& bias,
+                                  int out_type, const Tensor& status) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Normed n = rms_forward(x, opt(gain), eps, opt(residual), -1, true, false);
+  const Codes w = operand_of(w_codes, w_scales, w_square);
+  return py::make_tuple(give(product(n.codes->operand(), describe(w), w.cols, opt(bias), out_type, with_last(x, w.rows), x, status)),
+                        give(n.sum));
+}
+
+Tensor py_scaled_linear(const Tensor& x, const Tensor& w, const Optional& b, int out_type, bool need_x, bool need_w,
+                        const Tensor& status) {
+  return ScaledLinear::apply(x, w, b, static_cast<int64_t>(out_type), need_x, need_w, status);
+}
+py::tuple pair_of(const variable_list& v) { return py::make_tuple(give(v[0]), v.size() > 1 ? give(v[1]) : py::none()); }
+py::tuple py_rms_norm(const Tensor& x, const Optional& gain, const Optional& residual, double eps,
+                      int y_type, bool need) {
+  return pair_of(RmsNorm::apply(x, gain, residual, eps, static_cast<int64_t>(y_type), need));
+}
+py::tuple py_rms_norm_linear(const Tensor& x, const Optional& gain, const Tensor& w, const Optional& b,
+                             const Optional& residual, double eps, int out_type, bool need_h, bool need_w,
+                             const Tensor& status) {
+  return pair_of(RmsNormLinear::apply(x, gain, w, b, residual, eps, static_cast<int64_t>(out_type), need_h, need_w, status));
+}
+
+void init(const py::dict& entry) {
+  auto take = [&](auto& slot, const char* name) {
+    slot = reinterpret_cast<std::decay_t<decltype(slot)>>(entry[name].cast<uintptr_t>());
+  };
+  take(api.gemm, "jb_scaled_gemm");
+  take(api.quantize, "jb_quantize");
+  take(api.column_sum, "jb_column_sum");
+  take(api.rms_fwd, "jb_rms_norm_fwd");
+  take(api.rms_bwd_parts, "jb_rms_bwd_parts");
+  take(api.rms_bwd, "jb_rms_norm_bwd");
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_jb_torch, m) {
+  m.def("init", &init);
+  m.def("launches", [] { return launches.load(std::memory_order_relaxed); });
+  m.def("quantize", &py_quantize);
+  m.def("scaled_matmul", &py_scaled_matmul);
+  m.def("rms_quantize", &py_rms_quantize);
+  m.def("linear_prepared", &py_linear_prepared);
+  m.def("norm_linear_prepared", &py_norm_linear_prepared);
+  m.def("scaled_linear", &py_scaled_linear);
+  m.def("rms_norm", &py_rms_norm);
+  m.def("rms_norm_linear", &py_rms_norm_linear);
+}
