@@ -69,7 +69,7 @@ int jb_scaled_gemm(const JbScaledOperand* a, const JbScaledOperand* b, long long
 int jb_quantize(const JbQuant* q, void* stream);
 int jb_column_sum(const float* part, int P, int C, void* out, int out_type, void* stream);
 int jb_rms_max_cols();
-int jb_rms_norm_fwd(const JbRms* q, void* stream);
+int jb_rms_norm_fwd(const JbRms* q, int sm_count, void* stream);
 int jb_rms_bwd_parts(int rows, int cols, int sm_count);
 int jb_rms_norm_bwd(const JbRmsBwd* q, int sm_count, void* stream);
 }

@@ -15,10 +15,14 @@
 namespace jb {
 
 // ---------------------------------------------------------------- values and codes
-// The magnitude of a value as an integer that orders like it; 0 for infinities and NaN.
+// Magnitudes are compared as integers: the bits of a float without its sign order like the numbers, infinities and NaN above
+// all of them.  A block whose largest magnitude is below INF_BITS holds finite values only, and its codes need no checks;
+// otherwise the largest finite magnitude is found again, one value at a time.
+constexpr uint32_t INF_BITS = 0x7f800000u;
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ uint32_t finite_magnitude(float v) {
-  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-  return b < 0x7f800000u ? b : 0u;
+  const uint32_t b = magnitude(v);
+  return b < INF_BITS ? b : 0u;
 }
 // e8m0 byte of the scale of a block whose largest finite magnitude has these bits: 1.75 * 2^(e - 127) >= A with the
 // least e (adding 0x1fffff carries into the exponent exactly when the fraction is above .75), then 448 = 1.75 * 2^8.
@@ -28,14 +32,42 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t magnitude) {
   return static_cast<uint32_t>(e < 11 ? 11 : e);
 }
 __device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+template <bool CHECKED>
 __device__ __forceinline__ float code_input(float v, float inv) {
   const float q = v * inv;
-  return (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u ? q : __uint_as_float(0x7fffffffu);
+  if constexpr (CHECKED) return magnitude(v) < INF_BITS ? q : __uint_as_float(0x7fffffffu);
+  return q;
 }
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
   return lo | (hi << 16);
+}
+template <bool CHECKED>
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], float inv) {
+  return make_uint2(codes4(code_input<CHECKED>(v[0], inv), code_input<CHECKED>(v[1], inv), code_input<CHECKED>(v[2], inv), code_input<CHECKED>(v[3], inv)),
+                    codes4(code_input<CHECKED>(v[4], inv), code_input<CHECKED>(v[5], inv), code_input<CHECKED>(v[6], inv), code_input<CHECKED>(v[7], inv)));
+}
+// Scale byte and codes of a block of 128 values held by 16 neighbouring lanes, eight each.
+__device__ __forceinline__ uint32_t block_of_16_lanes(const float (&v)[8], uint2& codes) {
+  uint32_t m = 0u;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max(m, magnitude(v[e]));
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (__any_sync(0xffffffffu, m >= INF_BITS)) {
+    m = 0u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, finite_magnitude(v[e]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const uint32_t byte = scale_byte(m);
+    codes = codes8<true>(v, inverse_scale(byte));
+    return byte;
+  }
+  const uint32_t byte = scale_byte(m);
+  codes = codes8<false>(v, inverse_scale(byte));
+  return byte;
 }
 
 template <typename T> __device__ __forceinline__ float to_f32(T v);
@@ -89,6 +121,13 @@ __device__ __forceinline__ void store_vec(T* p, int live, const float (&v)[N]) {
   }
 }
 
+__device__ __forceinline__ float gain_at(const void* gain, int type, int c) {
+  if (gain == nullptr) return 1.f;
+  if (type == 1) return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(gain) + c));
+  if (type == 2) return __half2float(__ldg(static_cast<const __half*>(gain) + c));
+  return __ldg(static_cast<const float*>(gain) + c);
+}
+
 // ---------------------------------------------------------------- rows in blocks of 1 x 128
 struct QuantArgs {
   const void* x;
@@ -132,19 +171,9 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const long long row = row0 + 2 * (i0 + i) + (lane >> 4);
-        uint32_t m = 0u;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m = max(m, finite_magnitude(v[i][e]));
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const uint32_t byte = scale_byte(m);
-        const float inv = inverse_scale(byte);
-        if (row < a.rows && col < a.pitch) {
-          uint2 q;
-          q.x = codes4(code_input(v[i][0], inv), code_input(v[i][1], inv), code_input(v[i][2], inv), code_input(v[i][3], inv));
-          q.y = codes4(code_input(v[i][4], inv), code_input(v[i][5], inv), code_input(v[i][6], inv), code_input(v[i][7], inv));
-          *reinterpret_cast<uint2*>(a.codes + row * a.pitch + col) = q;
-        }
+        uint2 q;
+        const uint32_t byte = block_of_16_lanes(v[i], q);
+        if (row < a.rows && col < a.pitch) *reinterpret_cast<uint2*>(a.codes + row * a.pitch + col) = q;
         // row 2 (i0 + i) + h was reduced by lanes 16 h .. 16 h + 15
         const uint32_t other = __shfl_xor_sync(0xffffffffu, byte, 16);
         if ((lane >> 1) == i0 + i) mine = (lane & 1) == (lane >> 4) ? byte : other;
@@ -156,124 +185,167 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
 }
 
 // ---------------------------------------------------------------- tiles of 128 x 128
-// One CTA, one tile: values in registers (warp w: rows 16 w .. 16 w + 15, lane l: columns 4 l .. 4 l + 3), scales by
-// row (shuffles), by column (shared memory) or of the whole tile; the transposed codes turn in shared memory, 16 bytes
-// of one column at a time.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) quant_tile_kernel(const QuantArgs a) {
-  __shared__ __align__(16) uint8_t turned[128 * 128];
-  __shared__ uint32_t col_mag[8][128];
-  __shared__ float col_sum[8][128];
-  __shared__ uint32_t row_mag[8];
+// max(m, |a|, |b|), NaN if one of them is.
+__device__ __forceinline__ float max_abs3(float m, float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+
+struct TileShared {
+  __align__(16) uint8_t turned[128 * 128];
+  __align__(16) uint32_t col_mag[16][128];
+  __align__(16) float col_sum[16][128];
+  __align__(16) float col_inv[128];
+  uint32_t row_mag[16];
+};
+
+// One CTA, one tile, 32 values a thread (warp w: rows 8 w .. 8 w + 7, lane l: columns 4 l .. 4 l + 3), so that two CTAs of
+// sixteen warps share an SM.  Scales by row come from warp reductions, by column through shared memory, or from the
+// whole tile; the transposed codes turn in shared memory, eight bytes of a column at a time.
+template <typename T, bool VEC, bool NORM>
+__global__ void __launch_bounds__(512, 2) quant_tile_kernel(const QuantArgs a) {
+  __shared__ TileShared sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tile_r = blockIdx.x, tile_c = blockIdx.y;
-  const long long row0 = static_cast<long long>(tile_r) * 128 + warp * 16;
+  const long long row0 = static_cast<long long>(tile_r) * 128 + warp * 8;
   const int col = tile_c * 128 + lane * 4;
   const int live = min(4, max(0, a.cols - col));
-  const T* x = static_cast<const T*>(a.x);
-  float v[16][4];
+  const int live_rows = static_cast<int>(max(0LL, min(8LL, a.rows - row0)));
+  float v[8][4];
+  {
+    const T* x = static_cast<const T*>(a.x) + row0 * a.ldx + col;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) load_vec<T, 4, VEC>(x + (row0 + i) * a.ldx + col, row0 + i < a.rows ? live : 0, v[i]);
-  if (a.rstd != nullptr) {
-    float g[4];
+    for (int i = 0; i < 8; ++i) load_vec<T, 4, VEC>(x + i * a.ldx, i < live_rows ? live : 0, v[i]);
+  }
+  if constexpr (NORM) {
+    float g[4] = {1.f, 1.f, 1.f, 1.f};
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      g[j] = (a.gain == nullptr || j >= live) ? 1.f
-             : a.gain_type == 1 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.gain)[col + j])
-             : a.gain_type == 2 ? __half2float(static_cast<const __half*>(a.gain)[col + j])
-                                : static_cast<const float*>(a.gain)[col + j];
+      if (j < live) g[j] = gain_at(a.gain, a.gain_type, col + j);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float r = row0 + i < a.rows ? __ldg(a.rstd + row0 + i) : 0.f;
+    for (int i = 0; i < 8; ++i) {
+      const float r = i < live_rows ? __ldg(a.rstd + row0 + i) : 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[i][j] = v[i][j] * r * g[j];
     }
   }
-  uint32_t cm[4] = {0u, 0u, 0u, 0u};
+  uint32_t cm[4];
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
+  for (int j = 0; j < 4; ++j) {
+    float m = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) cm[j] = max(cm[j], finite_magnitude(v[i][j]));
+    for (int i = 0; i < 8; i += 2) m = max_abs3(m, v[i][j], v[i + 1][j]);
+    cm[j] = magnitude(m);
+  }
   if (a.colsum != nullptr) {
+    float t[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float t = 0.f;
+      t[j] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) t += v[i][j];
-      col_sum[warp][lane * 4 + j] = t;
+      for (int i = 0; i < 8; ++i) t[j] += v[i][j];
     }
+    *reinterpret_cast<float4*>(&sh.col_sum[warp][lane * 4]) = make_float4(t[0], t[1], t[2], t[3]);
   }
-  if (a.square) {
-    uint32_t m = max(max(cm[0], cm[1]), max(cm[2], cm[3]));
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (lane == 0) row_mag[warp] = m;
-  } else if (a.codes_t != nullptr) {
-    *reinterpret_cast<uint4*>(&col_mag[warp][lane * 4]) = make_uint4(cm[0], cm[1], cm[2], cm[3]);
-  }
-  __syncthreads();
-  if (a.colsum != nullptr && threadIdx.x < 128 && tile_c * 128 + threadIdx.x < a.cols) {
-    float t = 0.f;
+  const uint32_t top = max(max(cm[0], cm[1]), max(cm[2], cm[3]));
+  auto share = [&](uint32_t most) {
+    if (a.square) {
+      const uint32_t m = __reduce_max_sync(0xffffffffu, most);
+      if (lane == 0) sh.row_mag[warp] = m;
+    } else if (a.codes_t != nullptr) {
+      *reinterpret_cast<uint4*>(&sh.col_mag[warp][lane * 4]) = make_uint4(cm[0], cm[1], cm[2], cm[3]);
+    }
+  };
+  share(top);
+  // not a number among the values: the rest of the tile runs on finite magnitudes, and such values leave as NaN codes
+  const bool checked = __syncthreads_or(top >= INF_BITS) != 0;
+  if (checked) {
 #pragma unroll
-    for (int w = 0; w < 8; ++w) t += col_sum[w][threadIdx.x];
-    a.colsum[static_cast<long long>(tile_r) * a.cols + tile_c * 128 + threadIdx.x] = t;
+    for (int j = 0; j < 4; ++j) {
+      cm[j] = 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) cm[j] = max(cm[j], finite_magnitude(v[i][j]));
+    }
+    share(max(max(cm[0], cm[1]), max(cm[2], cm[3])));
+    __syncthreads();
   }
-
   uint32_t square_byte = 0u;
   if (a.square) {
     uint32_t m = 0u;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) m = max(m, row_mag[w]);
+    for (int w = 0; w < 16; ++w) m = max(m, sh.row_mag[w]);
     square_byte = scale_byte(m);
     if (threadIdx.x == 0) a.scales[tile_r * a.scale_row + tile_c * a.scale_k] = static_cast<uint8_t>(square_byte);
+  } else if (a.codes_t != nullptr && threadIdx.x < 128) {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) m = max(m, sh.col_mag[w][threadIdx.x]);
+    const uint32_t byte = scale_byte(m);
+    sh.col_inv[threadIdx.x] = inverse_scale(byte);
+    const int c = tile_c * 128 + threadIdx.x;
+    if (c < a.cols) a.scales_t[c * a.scale_t_row + tile_r * a.scale_t_k] = static_cast<uint8_t>(byte);
+  }
+  if (a.colsum != nullptr && threadIdx.x >= 128 && threadIdx.x < 256 && tile_c * 128 + threadIdx.x - 128 < a.cols) {
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) t += sh.col_sum[w][threadIdx.x - 128];
+    a.colsum[static_cast<long long>(tile_r) * a.cols + tile_c * 128 + threadIdx.x - 128] = t;
+  }
+  if (checked) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = code_input<true>(v[i][j], 1.f);      // NaN for every value that is not finite
   }
   if (a.codes != nullptr) {
     uint32_t mine = 0u;
+    uint8_t* out = a.codes + row0 * a.pitch + col;
+    const bool in_pitch = col < a.pitch;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
       uint32_t byte = square_byte;
       if (!a.square) {
-        uint32_t m = max(max(finite_magnitude(v[i][0]), finite_magnitude(v[i][1])), max(finite_magnitude(v[i][2]), finite_magnitude(v[i][3])));
+        uint32_t m = magnitude(max_abs3(max_abs3(0.f, v[i][0], v[i][1]), v[i][2], v[i][3]));
+        if (checked)
+          m = max(max(finite_magnitude(v[i][0]), finite_magnitude(v[i][1])), max(finite_magnitude(v[i][2]), finite_magnitude(v[i][3])));
         byte = scale_byte(__reduce_max_sync(0xffffffffu, m));
         if (lane == i) mine = byte;
       }
       const float inv = inverse_scale(byte);
-      if (row0 + i < a.rows && col < a.pitch)
-        *reinterpret_cast<uint32_t*>(a.codes + (row0 + i) * a.pitch + col) =
-            codes4(code_input(v[i][0], inv), code_input(v[i][1], inv), code_input(v[i][2], inv), code_input(v[i][3], inv));
+      if (i < live_rows && in_pitch)
+        *reinterpret_cast<uint32_t*>(out) = codes4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+      out += a.pitch;
     }
-    if (!a.square && lane < 16 && row0 + lane < a.rows)
-      a.scales[(row0 + lane) * a.scale_row + tile_c * a.scale_k] = static_cast<uint8_t>(mine);
+    if (!a.square && lane < live_rows) a.scales[(row0 + lane) * a.scale_row + tile_c * a.scale_k] = static_cast<uint8_t>(mine);
   }
   if (a.codes_t != nullptr) {
+    float inv[4];
+    if (a.square) {
+      inv[0] = inv[1] = inv[2] = inv[3] = inverse_scale(square_byte);
+    } else {
+      __syncthreads();
+      const float4 f = *reinterpret_cast<const float4*>(&sh.col_inv[lane * 4]);
+      inv[0] = f.x; inv[1] = f.y; inv[2] = f.z; inv[3] = f.w;
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      uint32_t byte = square_byte;
-      if (!a.square) {
-        uint32_t m = 0u;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) m = max(m, col_mag[w][lane * 4 + j]);
-        byte = scale_byte(m);
-        if (warp == j && col + j < a.cols)      // each warp writes one of the four
-          a.scales_t[(col + j) * a.scale_t_row + tile_r * a.scale_t_k] = static_cast<uint8_t>(byte);
-      }
-      const float inv = inverse_scale(byte);
-      uint4 q;
-      q.x = codes4(code_input(v[0][j], inv), code_input(v[1][j], inv), code_input(v[2][j], inv), code_input(v[3][j], inv));
-      q.y = codes4(code_input(v[4][j], inv), code_input(v[5][j], inv), code_input(v[6][j], inv), code_input(v[7][j], inv));
-      q.z = codes4(code_input(v[8][j], inv), code_input(v[9][j], inv), code_input(v[10][j], inv), code_input(v[11][j], inv));
-      q.w = codes4(code_input(v[12][j], inv), code_input(v[13][j], inv), code_input(v[14][j], inv), code_input(v[15][j], inv));
-      const int c = lane * 4 + j;
-      *reinterpret_cast<uint4*>(turned + c * 128 + ((warp ^ (lane & 7)) << 4)) = q;       // lane & 7 = (c >> 2) & 7
+      uint2 q;
+      q.x = codes4(v[0][j] * inv[j], v[1][j] * inv[j], v[2][j] * inv[j], v[3][j] * inv[j]);
+      q.y = codes4(v[4][j] * inv[j], v[5][j] * inv[j], v[6][j] * inv[j], v[7][j] * inv[j]);
+      // piece `warp` of column 4 lane + j, at a place that differs between the sixteen lanes of a store's half warp
+      *reinterpret_cast<uint2*>(sh.turned + (lane * 4 + j) * 128 + ((warp ^ (lane & 15)) << 3)) = q;
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = warp * 16 + i * 4 + (lane >> 3);
-      const int piece = lane & 7;
+    for (int i = 0; i < 2; ++i) {
+      const int c = warp * 8 + i * 4 + (lane >> 3);
+      const int piece = lane & 7, turn = (c >> 2) & 15;
+      uint4 q = *reinterpret_cast<const uint4*>(sh.turned + c * 128 + ((((2 * piece) ^ turn) & ~1) << 3));
+      if (turn & 1) q = make_uint4(q.z, q.w, q.x, q.y);
       const long long at = static_cast<long long>(tile_r) * 128 + piece * 16;
       if (tile_c * 128 + c < a.cols && at < a.pitch_t)
-        *reinterpret_cast<uint4*>(a.codes_t + (static_cast<long long>(tile_c) * 128 + c) * a.pitch_t + at) =
-            *reinterpret_cast<const uint4*>(turned + c * 128 + ((piece ^ ((c >> 2) & 7)) << 4));
+        *reinterpret_cast<uint4*>(a.codes_t + (static_cast<long long>(tile_c) * 128 + c) * a.pitch_t + at) = q;
     }
   }
 }
@@ -316,75 +388,106 @@ struct RmsArgs {
   long long scale_row, scale_k;
 };
 
-__device__ __forceinline__ float gain_at(const void* gain, int type, int c) {
-  if (gain == nullptr) return 1.f;
-  if (type == 1) return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(gain) + c));
-  if (type == 2) return __half2float(__ldg(static_cast<const __half*>(gain) + c));
-  return __ldg(static_cast<const float*>(gain) + c);
-}
-__device__ __forceinline__ void gain_vec(const void* gain, int type, int c, int live, bool vec, float (&g)[8]) {
-  if (gain != nullptr && vec && live == 8) {
-    if (type == 1) return load_vec<__nv_bfloat16, 8, true>(static_cast<const __nv_bfloat16*>(gain) + c, 8, g);
-    if (type == 2) return load_vec<__half, 8, true>(static_cast<const __half*>(gain) + c, 8, g);
-    return load_vec<float, 8, true>(static_cast<const float*>(gain) + c, 8, g);
-  }
+// Eight elements of a row: VEC, consecutive ones at column c (all or none of them exist); otherwise one every `step`
+// columns from c on, so that the lanes of a warp read neighbouring elements whatever the alignment (or, step = 1,
+// consecutive ones one by one).
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_raw(const T* row, int c, int step, int cols, T (&v)[8]) {
+  if constexpr (VEC) {
+    if (c < cols) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) g[e] = e < live ? gain_at(gain, type, c + e) : 0.f;
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(v)[i] = make_uint4(0u, 0u, 0u, 0u);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e * step < cols ? row[c + e * step] : from_f32<T>(0.f);
+  }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* row, int c, int step, int cols, float (&v)[8]) {
+  __align__(16) T raw[8];
+  load_raw<T, VEC>(row, c, step, cols, raw);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = to_f32<T>(raw[e]);
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T* row, int c, int step, int cols, const float (&v)[8]) {
+  if constexpr (VEC) {
+    if (c < cols) {
+      __align__(16) T raw[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) raw[e] = from_f32<T>(v[e]);
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(row + c)[i] = reinterpret_cast<const uint4*>(raw)[i];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e * step < cols) row[c + e * step] = from_f32<T>(v[e]);
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void gain8(const void* gain, int type, int c, int step, int cols, float (&g)[8]) {
+  if (gain == nullptr) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = 1.f;
+  } else if (type == 1) {
+    load8<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16*>(gain), c, step, cols, g);
+  } else if (type == 2) {
+    load8<__half, VEC>(static_cast<const __half*>(gain), c, step, cols, g);
+  } else {
+    load8<float, VEC>(static_cast<const float*>(gain), c, step, cols, g);
+  }
 }
 
-// Sum of `v` over the G threads of a row (G a multiple of 32; `slot` separates the rows of a CTA).
-template <int G>
+// Sum over the threads of a row: one warp, or the whole CTA (`shared` holds a value per warp).
+template <bool WARP>
 __device__ __forceinline__ double row_sum(double v, double* shared) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if constexpr (G > 32) {
-    const int warp = threadIdx.x >> 5;
-    constexpr int W = G / 32;
-    if ((threadIdx.x & 31) == 0) shared[warp] = v;
+  if constexpr (!WARP) {
+    const int warps = blockDim.x >> 5;
+    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
     __syncthreads();
     v = 0.0;
-    const int first = warp / W * W;
-#pragma unroll
-    for (int w = 0; w < W; ++w) v += shared[first + w];
+    for (int w = 0; w < warps; ++w) v += shared[w];
   }
   return v;
 }
 
-// G threads a row, NV vectors of 8 values each (vector i of thread g starts at 8 (i G + g)); rows up to 8 G NV values
-// stay in registers between the sum of squares and the output, so that every byte is read once.  The squares of a
-// thread are added in fp32, the threads in fp64: the sum is good to the last bit of fp32 or nearly so, whatever the
-// length of the row.
-template <typename T, int G, int NV, bool VEC>
-__global__ void __launch_bounds__(G < 256 ? 256 : G) rms_fwd_kernel(const RmsArgs a) {
-  constexpr int THREADS = G < 256 ? 256 : G;
-  constexpr int ROWS = THREADS / G;
-  __shared__ double shared[THREADS / 32];
-  const int g = threadIdx.x % G;
-  const long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / G;
-  const bool in = row < a.rows;
+// A row belongs to one warp (WARP: eight rows a CTA) or to one CTA; a thread keeps NV vectors of eight values between the
+// sum of squares and the output, so that every byte is read once.  The squares of a thread are added in fp32, the
+// threads in fp64: the sum is good to the last bit of fp32 or nearly so, whatever the length of the row.
+template <typename T, int NV, bool VEC, bool WARP, bool CODES, int MOST>
+__global__ void __launch_bounds__(MOST) rms_fwd_kernel(const RmsArgs a) {
+  __shared__ double shared[32];
+  const int G = WARP ? 32 : blockDim.x;                          // threads of a row
+  const int g = WARP ? (threadIdx.x & 31) : threadIdx.x;
+  const long long row = WARP ? static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
+  if (WARP && row >= a.rows) return;
+  // consecutive values per thread where blocks of 128 columns have to meet in 16 neighbouring lanes, or loads are wide
+  constexpr bool RUN = VEC || CODES;
+  const int step = RUN ? 1 : G;
+  auto column = [&](int i) { return RUN ? (i * G + g) * 8 : i * 8 * G + g; };
   const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-  const T* res = a.residual == nullptr ? nullptr : static_cast<const T*>(a.residual) + row * a.ldr;
   float t[NV][8];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * G + g) * 8;
-    load_vec<T, 8, VEC>(x + c, in ? min(8, max(0, a.cols - c)) : 0, t[i]);
-  }
-  if (res != nullptr) {
-    float r[NV][8];
+  for (int i = 0; i < NV; ++i) load8<T, VEC>(x, column(i), step, a.cols, t[i]);
+  if (a.residual != nullptr) {
+    const T* res = static_cast<const T*>(a.residual) + row * a.ldr;
+    __align__(16) T r[NV][8];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * G + g) * 8;
-      load_vec<T, 8, VEC>(res + c, in ? min(8, max(0, a.cols - c)) : 0, r[i]);
-    }
+    for (int i = 0; i < NV; ++i) load_raw<T, VEC>(res, column(i), step, a.cols, r[i]);
     T* sum = static_cast<T*>(a.sum) + row * a.cols;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * G + g) * 8;
       // the norm is of the sum as it is stored: the backward pass, which reads the stored one, differentiates this function
 #pragma unroll
-      for (int e = 0; e < 8; ++e) t[i][e] = to_f32<T>(from_f32<T>(t[i][e] + r[i][e]));
-      store_vec<T, 8, VEC>(sum + c, in ? min(8, max(0, a.cols - c)) : 0, t[i]);
+      for (int e = 0; e < 8; ++e) t[i][e] = to_f32<T>(from_f32<T>(t[i][e] + to_f32<T>(r[i][e])));
+      store8<T, VEC>(sum, column(i), step, a.cols, t[i]);
     }
   }
   float sq = 0.f;
@@ -392,92 +495,93 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) rms_fwd_kernel(const RmsArg
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) sq = fmaf(t[i][e], t[i][e], sq);
-  const double mean = row_sum<G>(static_cast<double>(sq), shared) / a.cols;
+  const double mean = row_sum<WARP>(static_cast<double>(sq), shared) / a.cols;
   const float rstd = static_cast<float>(1.0 / sqrt(mean + static_cast<double>(a.eps)));
-  if (a.rstd != nullptr && g == 0 && in) a.rstd[row] = rstd;
+  if (a.rstd != nullptr && g == 0) a.rstd[row] = rstd;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * G + g) * 8;
-    const int live = in ? min(8, max(0, a.cols - c)) : 0;
+    const int c = column(i);
     float w[8];
-    gain_vec(a.gain, a.gain_type, c, live, VEC, w);
+    gain8<VEC>(a.gain, a.gain_type, c, step, a.cols, w);
 #pragma unroll
     for (int e = 0; e < 8; ++e) t[i][e] = t[i][e] * rstd * w[e];
-    if (a.y != nullptr) {
-      const long long at = row * a.cols + c;
-      if (a.y_type == 0) store_vec<float, 8, VEC>(static_cast<float*>(a.y) + at, live, t[i]);
-      else store_vec<T, 8, VEC>(static_cast<T*>(a.y) + at, live, t[i]);
-    }
-    if (a.codes != nullptr) {
-      uint32_t m = 0u;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = max(m, finite_magnitude(t[i][e]));
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));   // 16 lanes = 128 columns
-      const uint32_t byte = scale_byte(m);
-      const float inv = inverse_scale(byte);
-      if (in && c < a.pitch) {
-        uint2 q;
-        q.x = codes4(code_input(t[i][0], inv), code_input(t[i][1], inv), code_input(t[i][2], inv), code_input(t[i][3], inv));
-        q.y = codes4(code_input(t[i][4], inv), code_input(t[i][5], inv), code_input(t[i][6], inv), code_input(t[i][7], inv));
-        *reinterpret_cast<uint2*>(a.codes + row * a.pitch + c) = q;
-      }
-      if (in && (g & 15) == 0 && c < a.cols) a.scales[row * a.scale_row + (c >> 7) * a.scale_k] = static_cast<uint8_t>(byte);
+    if constexpr (CODES) {
+      uint2 q;
+      const uint32_t byte = block_of_16_lanes(t[i], q);          // 16 lanes = 128 columns
+      if (c < a.pitch) *reinterpret_cast<uint2*>(a.codes + row * a.pitch + c) = q;
+      if ((g & 15) == 0 && c < a.cols) a.scales[row * a.scale_row + (c >> 7) * a.scale_k] = static_cast<uint8_t>(byte);
+    } else {
+      if (a.y_type == 0) store8<float, VEC>(static_cast<float*>(a.y) + row * a.cols, c, step, a.cols, t[i]);
+      else store8<T, VEC>(static_cast<T*>(a.y) + row * a.cols, c, step, a.cols, t[i]);
     }
   }
 }
 
-// dx = r (w g - t r^2 mean(w g t)) + gsum and the gain's gradient sum_rows g t r.  A CTA keeps the gain's partial sums
-// of its rows in registers and writes them once at the end; column_sum_kernel adds the CTAs' rows in a fixed order.
+// dx = r (w g - t r^2 mean(w g t)) + gsum and the gain's gradient sum_rows g t r.  A CTA takes rows in steps of the grid
+// and keeps the gain's partial sums of its columns in registers until the end; column_sum_kernel adds the CTAs' parts in
+// a fixed order.  The next row is read before the present one is worked on: with one row in flight the pass waited for
+// memory most of the time (16384 x 4096 bf16: 230 us, against 82 us of traffic).
 struct RmsBwdArgs {
   const void* t;             // the normalised sum, contiguous rows ldt apart
   long long ldt;
   const void* g;             // gradient of y: type of t, or fp32
-  int g_f32;
   const void* gsum;          // gradient of the sum, type of t, contiguous, or null
   const float* rstd;
   const void* gain;
   int gain_type;
   int rows, cols;
   void* dx;                  // contiguous
-  float* part;               // [gridDim.x * ROWS, cols], or null
+  float* part;               // [gridDim.x * rows of a CTA, cols], or null
 };
 
-template <typename T, int G, int NV, bool VEC>
-__global__ void __launch_bounds__(G < 256 ? 256 : G) rms_bwd_kernel(const RmsBwdArgs a) {
-  constexpr int THREADS = G < 256 ? 256 : G;
-  constexpr int ROWS = THREADS / G;
-  __shared__ double shared[2][THREADS / 32];
-  const int g = threadIdx.x % G;
-  const int lane_row = threadIdx.x / G;
+// MOST: threads of the largest CTA (registers: 128 a thread up to 512 threads, 64 beyond).
+template <typename T, typename TG, int NV, bool VEC, bool WARP, int MOST>
+__global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) rms_bwd_kernel(const RmsBwdArgs a) {
+  __shared__ double shared[2][32];
+  const int G = WARP ? 32 : blockDim.x;
+  const int g = WARP ? (threadIdx.x & 31) : threadIdx.x;
+  const long long first = WARP ? static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
+  const long long stride = static_cast<long long>(gridDim.x) * (WARP ? 8 : 1);
+  const int step = VEC ? 1 : G;
+  auto column = [&](int i) { return VEC ? (i * G + g) * 8 : i * 8 * G + g; };
+  const T* ts = static_cast<const T*>(a.t);
+  const TG* gs = static_cast<const TG*>(a.g);
+  const T* ss = static_cast<const T*>(a.gsum);
+  T* dxs = static_cast<T*>(a.dx);
   float dw[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[i][e] = 0.f;
-  int turn = 0;
-  const long long stride = static_cast<long long>(gridDim.x) * ROWS;
-  const long long rounds = (a.rows + stride - 1) / stride;       // the same for every thread: row_sum has barriers
-  for (long long k = 0; k < rounds; ++k, turn ^= 1) {
-    const long long row = k * stride + static_cast<long long>(blockIdx.x) * ROWS + lane_row;
-    const bool in = row < a.rows;
-    float t[NV][8], y[NV][8];
+  __align__(16) T nt[NV][8], ns[NV][8];
+  __align__(16) TG ng[NV][8];
+  auto fetch = [&](long long row) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * G + g) * 8;
-      const int live = in ? min(8, max(0, a.cols - c)) : 0;
-      load_vec<T, 8, VEC>(static_cast<const T*>(a.t) + row * a.ldt + c, live, t[i]);
-      if (a.g_f32) load_vec<float, 8, VEC>(static_cast<const float*>(a.g) + row * a.cols + c, live, y[i]);
-      else load_vec<T, 8, VEC>(static_cast<const T*>(a.g) + row * a.cols + c, live, y[i]);
+      load_raw<T, VEC>(ts + row * a.ldt, column(i), step, a.cols, nt[i]);
+      load_raw<TG, VEC>(gs + row * a.cols, column(i), step, a.cols, ng[i]);
+      if (ss != nullptr) load_raw<T, VEC>(ss + row * a.cols, column(i), step, a.cols, ns[i]);
     }
-    const float r = in ? __ldg(a.rstd + row) : 0.f;
+  };
+  if (first < a.rows) fetch(first);
+  int turn = 0;
+  for (long long row = first; row < a.rows; row += stride, turn ^= 1) {     // the same trip count for all threads of a row
+    float t[NV][8], y[NV][8], s[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        t[i][e] = to_f32<T>(nt[i][e]);
+        y[i][e] = to_f32<TG>(ng[i][e]);
+        s[i][e] = ss != nullptr ? to_f32<T>(ns[i][e]) : 0.f;
+      }
+    const float r = __ldg(a.rstd + row);
+    if (row + stride < a.rows) fetch(row + stride);
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * G + g) * 8;
-      const int live = in ? min(8, max(0, a.cols - c)) : 0;
       float w[8];
-      gain_vec(a.gain, a.gain_type, c, live, VEC, w);
+      gain8<VEC>(a.gain, a.gain_type, column(i), step, a.cols, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         dw[i][e] = fmaf(y[i][e], t[i][e] * r, dw[i][e]);
@@ -485,70 +589,64 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) rms_bwd_kernel(const RmsBwd
         dot = fmaf(y[i][e], t[i][e], dot);
       }
     }
-    const float inner = static_cast<float>(row_sum<G>(static_cast<double>(dot), shared[turn]) / a.cols);
+    const float inner = static_cast<float>(row_sum<WARP>(static_cast<double>(dot), shared[turn]) / a.cols);
     const float k3 = r * r * inner;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * G + g) * 8;
-      const int live = in ? min(8, max(0, a.cols - c)) : 0;
-      float s[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] = 0.f;
-      if (a.gsum != nullptr) load_vec<T, 8, VEC>(static_cast<const T*>(a.gsum) + row * a.cols + c, live, s);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] = fmaf(r, y[i][e] - t[i][e] * k3, s[e]);
-      store_vec<T, 8, VEC>(static_cast<T*>(a.dx) + row * a.cols + c, live, s);
+      for (int e = 0; e < 8; ++e) s[i][e] = fmaf(r, y[i][e] - t[i][e] * k3, s[i][e]);
+      store8<T, VEC>(dxs + row * a.cols, column(i), step, a.cols, s[i]);
     }
   }
   if (a.part != nullptr) {
-    float* out = a.part + (static_cast<long long>(blockIdx.x) * ROWS + lane_row) * a.cols;
+    float* out = a.part + first * a.cols;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * G + g) * 8;
-      store_vec<float, 8, VEC>(out + c, min(8, max(0, a.cols - c)), dw[i]);
-    }
+    for (int i = 0; i < NV; ++i) store8<float, VEC>(out, column(i), step, a.cols, dw[i]);
   }
 }
 
 // ---------------------------------------------------------------- dispatch
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Threads per row when each keeps `held` values: a row of up to 1024 * held stays in registers.
-static inline int rms_group(int cols, int held) {
-  int g = 32;
-  while (g < 1024 && g * held < cols) g *= 2;
-  return g;
-}
-// Forward: 32 values a thread (60 registers).  Backward: 16, because it holds three arrays (row, gradient, partial sums
-// of the gain); rows beyond 16384 take 32 and spill.
-constexpr int RMS_FWD_HELD = 32;
-static inline int rms_bwd_held(int cols) { return cols <= 16384 ? 16 : 32; }
+// Threads of a CTA that takes one row, `held` values each.
+static inline int rms_threads(int cols, int held) { return ((cols + held - 1) / held + 31) / 32 * 32; }
 
-template <typename T, bool VEC>
-static int launch_rms_fwd(const RmsArgs& a, cudaStream_t st) {
-#define JB_RMS_FWD(G)                                                                                          \
-  case G: {                                                                                                    \
-    constexpr int ROWS = (G < 256 ? 256 : G) / G;                                                              \
-    rms_fwd_kernel<T, G, 4, VEC><<<(a.rows + ROWS - 1) / ROWS, G < 256 ? 256 : G, 0, st>>>(a);                 \
-    break;                                                                                                     \
-  }
-  switch (rms_group(a.cols, RMS_FWD_HELD)) { JB_RMS_FWD(32) JB_RMS_FWD(64) JB_RMS_FWD(128) JB_RMS_FWD(256) JB_RMS_FWD(512) JB_RMS_FWD(1024) }
-#undef JB_RMS_FWD
+// Rows of up to 1024 values: a warp each.  Longer ones: a CTA each, 32 values a thread, or 8 where there are fewer rows
+// than SMs and the time is that of one row's chain of loads and sums (4096 bf16, one row: 4.5 us with 32 a thread).
+template <typename T, bool VEC, bool CODES>
+static int launch_rms_fwd(const RmsArgs& a, int sm_count, cudaStream_t st) {
+  const int warps = (a.rows + 7) / 8;
+  if (a.rows < sm_count && a.cols > 256 && a.cols <= 8192)
+    rms_fwd_kernel<T, 1, VEC, false, CODES, 1024><<<a.rows, rms_threads(a.cols, 8), 0, st>>>(a);
+  else if (a.cols <= 512) rms_fwd_kernel<T, 2, VEC, true, CODES, 256><<<warps, 256, 0, st>>>(a);
+  else if (a.cols <= 1024) rms_fwd_kernel<T, 4, VEC, true, CODES, 256><<<warps, 256, 0, st>>>(a);
+  else if (a.cols <= 16384) rms_fwd_kernel<T, 4, VEC, false, CODES, 512><<<a.rows, rms_threads(a.cols, 32), 0, st>>>(a);
+  else rms_fwd_kernel<T, 4, VEC, false, CODES, 1024><<<a.rows, rms_threads(a.cols, 32), 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
-template <typename T, bool VEC>
-static int launch_rms_bwd(const RmsBwdArgs& a, int grid, cudaStream_t st) {
-  if (rms_bwd_held(a.cols) == 32) {
-    rms_bwd_kernel<T, 1024, 4, VEC><<<grid, 1024, 0, st>>>(a);
-    return cudaGetLastError() == cudaSuccess ? 0 : -4;
-  }
-#define JB_RMS_BWD(G)                                                               \
-  case G:                                                                           \
-    rms_bwd_kernel<T, G, 2, VEC><<<grid, G < 256 ? 256 : G, 0, st>>>(a);            \
-    break;
-  switch (rms_group(a.cols, 16)) { JB_RMS_BWD(32) JB_RMS_BWD(64) JB_RMS_BWD(128) JB_RMS_BWD(256) JB_RMS_BWD(512) JB_RMS_BWD(1024) }
-#undef JB_RMS_BWD
+// Backward: a thread holds three arrays (row, gradient, partial sums of the gain) and the next row, 16 values of each up to
+// 8192 columns and 32 beyond; rows beyond 16384 take 1024 threads and spill.
+static inline bool rms_bwd_by_warp(int cols) { return cols <= 512; }
+static inline int rms_bwd_threads(int cols) {
+  return rms_bwd_by_warp(cols) ? 256 : rms_threads(cols, cols <= 8192 ? 16 : 32);
+}
+static inline int rms_bwd_ctas(int rows, int cols, int sm_count) {
+  const int threads = rms_bwd_threads(cols);
+  const int resident = threads > 256 ? 1 : 512 / threads < 8 ? 512 / threads : 8;
+  const long long want = rms_bwd_by_warp(cols) ? (static_cast<long long>(rows) + 7) / 8 : rows;
+  const long long most = static_cast<long long>(sm_count) * resident;
+  return static_cast<int>(want < most ? want : most);
+}
+
+template <typename T, typename TG, bool VEC>
+static int launch_rms_bwd(const RmsBwdArgs& a, int sm_count, cudaStream_t st) {
+  const int grid = rms_bwd_ctas(a.rows, a.cols, sm_count), threads = rms_bwd_threads(a.cols);
+  if (rms_bwd_by_warp(a.cols)) rms_bwd_kernel<T, TG, 2, VEC, true, 256><<<grid, threads, 0, st>>>(a);
+  else if (threads <= 256 && a.cols <= 8192) rms_bwd_kernel<T, TG, 2, VEC, false, 256><<<grid, threads, 0, st>>>(a);
+  else if (a.cols <= 8192) rms_bwd_kernel<T, TG, 2, VEC, false, 512><<<grid, threads, 0, st>>>(a);
+  else if (a.cols <= 16384) rms_bwd_kernel<T, TG, 4, VEC, false, 512><<<grid, threads, 0, st>>>(a);
+  else rms_bwd_kernel<T, TG, 4, VEC, false, 1024><<<grid, threads, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
@@ -560,8 +658,13 @@ static int launch_quant(const QuantArgs& a, bool tiles, cudaStream_t st) {
     const bool vec = a.cols % 4 == 0 && (a.ldx * size) % (4 * size) == 0 && (reinterpret_cast<uintptr_t>(a.x) & (4 * size - 1)) == 0;
     if (kblocks > 65535) return -1;
     const dim3 grid(rblocks, kblocks);
-    if (vec) quant_tile_kernel<T, true><<<grid, 256, 0, st>>>(a);
-    else quant_tile_kernel<T, false><<<grid, 256, 0, st>>>(a);
+    if (a.rstd != nullptr) {
+      if (vec) quant_tile_kernel<T, true, true><<<grid, 512, 0, st>>>(a);
+      else quant_tile_kernel<T, false, true><<<grid, 512, 0, st>>>(a);
+    } else {
+      if (vec) quant_tile_kernel<T, true, false><<<grid, 512, 0, st>>>(a);
+      else quant_tile_kernel<T, false, false><<<grid, 512, 0, st>>>(a);
+    }
   } else {
     const bool vec = a.cols % 8 == 0 && (a.ldx * size) % 16 == 0 && aligned16(a.x);
     if ((kblocks + 7) / 8 > 65535) return -1;
@@ -607,10 +710,10 @@ extern "C" int jb_column_sum(const float* part, int P, int C, void* out, int out
 // Longest row that the kernels keep in registers.
 extern "C" int jb_rms_max_cols() { return 32768; }
 
-extern "C" int jb_rms_norm_fwd(const JbRms* q, void* stream) {
+extern "C" int jb_rms_norm_fwd(const JbRms* q, int sm_count, void* stream) {
   using namespace jb;
-  if (q == nullptr || q->rows < 1 || q->cols < 1 || q->cols > jb_rms_max_cols()) return -1;
-  if ((q->residual == nullptr) != (q->sum == nullptr)) return -1;
+  if (q == nullptr || q->rows < 1 || q->cols < 1 || q->cols > jb_rms_max_cols() || q->type < 0 || q->type > 2) return -1;
+  if ((q->residual == nullptr) != (q->sum == nullptr) || (q->codes == nullptr) == (q->y == nullptr)) return -1;
   if (q->codes != nullptr && ((q->pitch & 15) || !aligned16(q->codes) || q->pitch < q->cols)) return -1;
   if (q->y != nullptr && q->y_type != 0 && q->y_type != q->type) return -1;
   RmsArgs a{};
@@ -622,40 +725,38 @@ extern "C" int jb_rms_norm_fwd(const JbRms* q, void* stream) {
   const bool vec = q->cols % 8 == 0 && (q->ldx * size) % 16 == 0 && (q->ldr * size) % 16 == 0 && aligned16(q->x) &&
                    aligned16(q->residual) && aligned16(q->sum) && aligned16(q->y) && aligned16(q->gain);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (q->type == 0) return vec ? launch_rms_fwd<float, true>(a, st) : launch_rms_fwd<float, false>(a, st);
-  if (q->type == 1) return vec ? launch_rms_fwd<__nv_bfloat16, true>(a, st) : launch_rms_fwd<__nv_bfloat16, false>(a, st);
-  if (q->type == 2) return vec ? launch_rms_fwd<__half, true>(a, st) : launch_rms_fwd<__half, false>(a, st);
-  return -1;
+#define JB_RMS(T)                                                                                              \
+  if (q->codes != nullptr) return vec ? launch_rms_fwd<T, true, true>(a, sm_count, st) : launch_rms_fwd<T, false, true>(a, sm_count, st); \
+  return vec ? launch_rms_fwd<T, true, false>(a, sm_count, st) : launch_rms_fwd<T, false, false>(a, sm_count, st);
+  if (q->type == 0) { JB_RMS(float) }
+  if (q->type == 1) { JB_RMS(__nv_bfloat16) }
+  JB_RMS(__half)
+#undef JB_RMS
 }
 
-// CTAs of the backward pass and rows of its partial sums.  Two CTAs an SM fill it; a CTA takes at least four rounds of
-// rows, so that the partial sums stay a small part of the traffic.
-extern "C" int jb_rms_bwd_grid(int rows, int cols, int sm_count) {
-  const int g = jb::rms_group(cols, jb::rms_bwd_held(cols));
-  const int per = (g < 256 ? 256 : g) / g;
-  const int most = sm_count * (g <= 256 ? 2 : 1);
-  const long long want = (static_cast<long long>(rows) + 4 * per - 1) / (4 * per);
-  return static_cast<int>(want < 1 ? 1 : (want < most ? want : most));
-}
+// Rows of the gain's partial sums that jb_rms_norm_bwd writes.
 extern "C" int jb_rms_bwd_parts(int rows, int cols, int sm_count) {
-  const int g = jb::rms_group(cols, jb::rms_bwd_held(cols));
-  return jb_rms_bwd_grid(rows, cols, sm_count) * ((g < 256 ? 256 : g) / g);
+  return jb::rms_bwd_ctas(rows, cols, sm_count) * (jb::rms_bwd_by_warp(cols) ? 8 : 1);
 }
 
 extern "C" int jb_rms_norm_bwd(const JbRmsBwd* q, int sm_count, void* stream) {
   using namespace jb;
-  if (q == nullptr || q->rows < 1 || q->cols < 1 || q->cols > jb_rms_max_cols()) return -1;
+  if (q == nullptr || q->rows < 1 || q->cols < 1 || q->cols > jb_rms_max_cols() || q->type < 0 || q->type > 2) return -1;
   RmsBwdArgs a{};
-  a.t = q->t; a.ldt = q->ldt; a.g = q->g; a.g_f32 = q->g_f32 || q->type == 0; a.gsum = q->gsum;
+  a.t = q->t; a.ldt = q->ldt; a.g = q->g; a.gsum = q->gsum;
   a.rstd = static_cast<const float*>(q->rstd); a.gain = q->gain; a.gain_type = q->gain_type; a.rows = q->rows; a.cols = q->cols;
   a.dx = q->dx; a.part = static_cast<float*>(q->part);
   const long long size = q->type == 0 ? 4 : 2;
   const bool vec = q->cols % 8 == 0 && (q->ldt * size) % 16 == 0 && aligned16(q->t) && aligned16(q->g) && aligned16(q->gsum) &&
                    aligned16(q->gain) && aligned16(q->dx) && aligned16(q->part);
-  const int grid = jb_rms_bwd_grid(q->rows, q->cols, sm_count);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (q->type == 0) return vec ? launch_rms_bwd<float, true>(a, grid, st) : launch_rms_bwd<float, false>(a, grid, st);
-  if (q->type == 1) return vec ? launch_rms_bwd<__nv_bfloat16, true>(a, grid, st) : launch_rms_bwd<__nv_bfloat16, false>(a, grid, st);
-  if (q->type == 2) return vec ? launch_rms_bwd<__half, true>(a, grid, st) : launch_rms_bwd<__half, false>(a, grid, st);
-  return -1;
+#define JB_RMS(T, TG) return vec ? launch_rms_bwd<T, TG, true>(a, sm_count, st) : launch_rms_bwd<T, TG, false>(a, sm_count, st);
+  if (q->type == 0) { JB_RMS(float, float) }
+  if (q->type == 1) {
+    if (q->g_f32) { JB_RMS(__nv_bfloat16, float) }
+    JB_RMS(__nv_bfloat16, __nv_bfloat16)
+  }
+  if (q->g_f32) { JB_RMS(__half, float) }
+  JB_RMS(__half, __half)
+#undef JB_RMS
 }

@@ -249,7 +249,7 @@ Normed rms_forward(const Tensor& input, const Tensor& gain, double eps, const Te
     q.scale_k = c.scale_k;
     out.codes = std::move(c);
   }
-  done(api.rms_fwd(&q, stream_of(x.t)), "rms_norm_fwd");
+  done(api.rms_fwd(&q, sm_count(x.t), stream_of(x.t)), "rms_norm_fwd");
   return out;
 }
 
