@@ -4,14 +4,21 @@
 //
 // a [M, K] and b [N, K] are e4m3 codes, K contiguous; a scale is one e8m0 byte (2^(byte - 127)) per 128 values of K
 // and per row, or per 128 rows.  tcgen05.mma applies the scales itself (kind::mxf8f6f4.block_scale, one scale per 32
-// values of K): every product of two codes and two scales is exact, and the sum stays in fp32 in TMEM from the first
-// k-block to the last.  The 128-wide block is handed to the instruction by writing each scale byte four times.
+// values of K): every product of two codes and two scales is exact, and the sum stays in fp32 in TMEM.  A TMEM word holds
+// the scale bytes of one row for four k-blocks; the four products of a k-block all name its byte.
 //
-// One CTA, twelve warps: warp 0 issues the TMA loads of the code tiles, warps 2 and 3 lay the scale bytes of the same
-// k-block out in shared memory in the form that tcgen05.cp copies to TMEM (row r of a 128-row group at byte
+// Twelve warps a CTA: warp 0 issues the TMA loads of the code tiles, warps 2 and 3 lay the scale words of four k-blocks
+// out in shared memory in the form that tcgen05.cp copies to TMEM (row r of a 128-row group at byte
 // (r % 32) * 16 + (r / 32) * 4), warp 1 issues the copies and the products, warps 4..11 drain.  The drain reads a
 // warp's whole share of the accumulator into registers and gives the TMEM columns back before it converts and stores,
 // so that the products of the next tile run under the stores.
+//
+// Three forms:
+//  * PAIR: two CTAs of a cluster share a tile of 256 rows (cta_group::2); each loads its 128 rows of one operand and
+//    half of the other, so that a k-block costs 32 KB of loads an SM instead of 48 KB.
+//  * JOIN: a tile's k-blocks are cut over the CTAs of a cluster; the parts are pushed into the shared memory of the CTA
+//    that finishes them and added in rank order.  For products with fewer tiles than SMs.
+//  * SWAP (with JOIN): few rows (a token, a short batch): the weight's rows go along the 128 lanes.
 #include <type_traits>
 
 #include "ptx.cuh"
@@ -21,42 +28,72 @@
 namespace jb {
 
 // ---------------------------------------------------------------- instructions of this kernel
-// Block-scaled instruction descriptor: e4m3 x e4m3, e8m0 scales (byte 0 of each TMEM word), fp32 accumulation, M = 128.
-__host__ __device__ constexpr uint32_t make_idesc_mxf8(uint32_t N) {
-  return ((N >> 3) << 17) | (1u << 23) | ((128u >> 7) << 27);
+// Block-scaled instruction descriptor: e4m3 x e4m3, e8m0 scales in byte `byte` of each TMEM word, fp32 accumulation, M = 128
+// or 256.
+__host__ __device__ constexpr uint32_t make_idesc_mxf8(uint32_t M, uint32_t N, uint32_t byte) {
+  return (byte << 4) | ((N >> 3) << 17) | (1u << 23) | ((M >> 7) << 27) | (byte << 29);
 }
+template <bool PAIR>
 __device__ __forceinline__ void umma_mxf8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
                                           uint32_t sfb, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-      : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
 }
-// 32 rows of 16 bytes -> 32 lanes x 4 columns, repeated in all four lane quadrants.
+// 32 rows of 16 bytes -> 32 lanes x 4 columns, repeated in all four lane quadrants (of each CTA, from its own shared memory).
+template <bool PAIR>
 __device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Arrive on the mbarrier (of both CTAs) once the tcgen05 work issued so far has finished.
+template <bool PAIR>
+__device__ __forceinline__ void sg_commit(uint64_t* bar) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3)) : "memory");
+  else umma_commit(bar);
+}
+// Arrive on the same mbarrier of the cluster's CTA 0.  What the arrival announces (tiles and scales in this CTA's own shared
+// memory, or TMEM columns read) is complete by then and is not read by the other CTA's threads, only by the tensor
+// cores; a release at cluster scope would wait for every store of the thread and cost 0.9 us a k-block.
+__device__ __forceinline__ void mbar_arrive_leader(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %0, 0;\n\t"
+      "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar)) : "memory");
 }
 // No swizzle: groups of eight 16-byte rows, 128 bytes apart.
 __device__ __forceinline__ uint64_t make_smem_desc_scales(uint32_t saddr) {
   return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) |
          (static_cast<uint64_t>(1) << 46);
 }
-__device__ __forceinline__ void cluster_arrive_wait() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t local_saddr, uint32_t rank) {
+// The address of the same shared-memory place in another CTA of the cluster, and a store there.
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t local_saddr, uint32_t rank) {
   uint32_t remote;
-  float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local_saddr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
-  return v;
+  return remote;
+}
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
 // ---------------------------------------------------------------- arguments
@@ -83,6 +120,7 @@ struct ScaledOperand {       // scales of one operand: byte of (row r, k-block k
   long long row, k;
   int shift;                 // 0: a scale per row, 7: per 128 rows
   int rows;
+  int words;                 // k = 1, base and `row` multiples of four: four k-blocks are one aligned word
 };
 struct ScaledGemmArgs {
   ScaledOperand p, q;        // the operand along the accumulator's lanes (128 rows a tile), and along its columns
@@ -92,34 +130,39 @@ struct ScaledGemmArgs {
   const void* bias;          // [N] or null
   int bias_type;
   int kblocks;               // blocks of 128 along K
+  int chunk;                 // k-blocks summed in TMEM before the drain adds them up
   int tiles_p, tiles_q;
   int vec_out;               // rows of the output start on 16-byte boundaries
 };
 
-constexpr int SG_BP = 128;
+constexpr int SG_BP = 128;                   // rows of the operand along the lanes, per CTA
 constexpr int SG_EPI_WARPS = 8;
 constexpr int SG_THREADS = 32 * (4 + SG_EPI_WARPS);
-constexpr int SG_PITCH = SG_BP + 1;          // floats between columns of a dumped accumulator
+constexpr int SG_PITCH = SG_BP + 1;          // floats between columns of a part in shared memory
 
-// BQ: columns of a tile.  JOIN: the accumulator goes through shared memory, where the CTAs of a cluster that share a
-// tile (each with its own range of k-blocks) add their parts in rank order.
-template <int BQ, bool JOIN>
+// BQ: columns of a tile.
+template <int BQ, bool PAIR, bool JOIN>
 struct SgSmem {
   static constexpr int Q_ATOMS = (BQ + 127) / 128;
+  static constexpr int Q_ROWS = PAIR ? BQ / 2 : BQ;                // rows of the second operand that this CTA loads
   static constexpr int P_BYTES = SG_BP * 128;
-  static constexpr int Q_BYTES = BQ * 128;
-  static constexpr int TILE_BYTES = P_BYTES + Q_BYTES;             // multiples of 1024: swizzled operands
-  static constexpr int SF_BYTES = 512 * (1 + Q_ATOMS);
-  static constexpr int STAGES = BQ >= 256 ? 4 : (BQ >= 128 ? 6 : 8);
+  static constexpr int TILE_BYTES = P_BYTES + Q_ROWS * 128;        // multiples of 1024: swizzled operands
+  static constexpr int SF_BYTES = 512 * (1 + Q_ATOMS);             // scale words of four k-blocks
+  static constexpr int SF_SLOTS = 3;
+  static constexpr int STAGES = TILE_BYTES >= 49152 ? 4 : TILE_BYTES >= 32768 ? (JOIN ? 4 : 6) : JOIN && BQ >= 64 ? 6 : 8;
   static constexpr int ACCS = BQ >= 256 ? 1 : 2;
   static constexpr int SF_OFFSET = STAGES * TILE_BYTES;
-  static constexpr int STAGE_OUT = SF_OFFSET + STAGES * SF_BYTES;  // 32 rows x 64 bytes per draining warp
-  static constexpr int BAR_OFFSET = STAGE_OUT + (JOIN ? 0 : SG_EPI_WARPS * 2048);
+  static constexpr int OUT_OFFSET = SF_OFFSET + SF_SLOTS * SF_BYTES;
+  // plain: 32 rows x 64 bytes per draining warp; JOIN: the parts of BQ / split columns from each CTA
+  static constexpr int OUT_BYTES = JOIN ? (BQ * SG_PITCH * 4 + 15) / 16 * 16 : SG_EPI_WARPS * 2048;
+  static constexpr int BAR_OFFSET = OUT_OFFSET + OUT_BYTES;
+  static constexpr int BARS = 2 * STAGES + 2 * SF_SLOTS + 2 * ACCS;
   static constexpr int TOTAL = BAR_OFFSET + 256 + 1024;
   static_assert(TOTAL <= 227 * 1024, "shared memory of one CTA");
-  static_assert(!JOIN || BQ * SG_PITCH * 4 <= SF_OFFSET, "the dumped accumulator reuses the tile buffers");
+  static_assert(BARS * 8 + 8 <= 256, "barriers");
   static constexpr int SF_COL = ACCS * BQ < 32 ? 32 : ACCS * BQ;   // first TMEM column of the scales
-  static_assert(SF_COL + STAGES * 4 * (1 + Q_ATOMS) <= 512, "TMEM columns");
+  static constexpr int SF_COLS = 4 * (1 + Q_ATOMS);
+  static_assert(SF_COL + SF_SLOTS * SF_COLS <= 512, "TMEM columns");
 };
 
 // Position of tile t: groups of eight tile rows, walked down first, so that the CTAs of one wave share operand tiles.
@@ -132,89 +175,144 @@ __device__ __forceinline__ void sg_tile(int t, int tiles_p, int tiles_q, int& tp
   tq = r / height;
 }
 
-// One warp writes the scale words of `atoms` groups of 128 rows for its share of k-blocks, four k-blocks of loads ahead
-// of the stores (the loads' latency is several times a stage's time).
-template <int ATOMS>
-__device__ __forceinline__ void sg_load_scales(const ScaledOperand& o, int row0, int kb, int kend, uint32_t (&w)[ATOMS * 4], int lane) {
+// Scale bytes of one row for the k-blocks kb .. kb + 3 (those below kend).
+__device__ __forceinline__ uint32_t sg_scale_word(const ScaledOperand& o, int r, int kb, int kend) {
+  const uint8_t* p = o.scales + static_cast<long long>(r >> o.shift) * o.row + kb * o.k;
+  if (o.words && kb + 4 <= kend) return __ldg(reinterpret_cast<const uint32_t*>(p));
+  uint32_t w = 0u;
 #pragma unroll
-  for (int j = 0; j < ATOMS * 4; ++j) {
-    const int r = row0 + 32 * j + lane;
-    w[j] = 127u;
-    if (r < o.rows && kb < kend) w[j] = __ldg(o.scales + static_cast<long long>(r >> o.shift) * o.row + kb * o.k);
+  for (int j = 0; j < 4; ++j)
+    if (kb + j < kend) w |= static_cast<uint32_t>(__ldg(p + j * o.k)) << (8 * j);
+  return w;
+}
+// The words of `ATOMS` groups of 128 rows from row0 on, lane l: rows l, 32 + l, 64 + l, 96 + l of each.  A group whose rows
+// share their scales (tiles start on multiples of their height, which divides 128 or is a multiple of it) is one word.
+template <int ATOMS>
+__device__ __forceinline__ void sg_scale_words(const ScaledOperand& o, int row0, int kb, int kend, uint32_t (&w)[ATOMS * 4], int lane) {
+#pragma unroll
+  for (int g = 0; g < ATOMS; ++g) {
+    if (o.shift != 0) {
+      const uint32_t v = row0 + 128 * g < o.rows && kb < kend ? sg_scale_word(o, row0 + 128 * g, kb, kend) : 0x7f7f7f7fu;
+      w[4 * g] = w[4 * g + 1] = w[4 * g + 2] = w[4 * g + 3] = v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = row0 + 128 * g + 32 * j + lane;
+        w[4 * g + j] = r < o.rows && kb < kend ? sg_scale_word(o, r, kb, kend) : 0x7f7f7f7fu;
+      }
+    }
   }
 }
 
-template <int BQ, bool SWAP, bool JOIN>
+template <int BQ, bool PAIR, bool SWAP, bool JOIN>
 __global__ void __launch_bounds__(SG_THREADS, 1)
 scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ, const ScaledGemmArgs a,
                    int* status) {
-  using S = SgSmem<BQ, JOIN>;
+  static_assert(!(PAIR && JOIN) && (JOIN || !SWAP), "forms");
+  using S = SgSmem<BQ, PAIR, JOIN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BAR_OFFSET);
-  uint64_t* full = bars;                               // [STAGES]: TMA bytes and two scale warps
+  uint64_t* full = bars;                               // [STAGES]: TMA bytes (and the other CTA's)
   uint64_t* empty = bars + S::STAGES;                  // [STAGES]
-  uint64_t* acc_full = bars + 2 * S::STAGES;           // [ACCS]
+  uint64_t* sf_full = bars + 2 * S::STAGES;            // [SF_SLOTS]: two scale warps (and the other CTA's two)
+  uint64_t* sf_empty = sf_full + S::SF_SLOTS;          // [SF_SLOTS]
+  uint64_t* acc_full = sf_empty + S::SF_SLOTS;         // [ACCS]
   uint64_t* acc_empty = acc_full + S::ACCS;            // [ACCS]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + S::ACCS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((2 * S::STAGES + 2 * S::ACCS) * 8 + 8 <= 256, "barriers");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t split = 1, rank = 0;
+  if constexpr (JOIN) asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(split));
+  if constexpr (JOIN || PAIR) rank = cluster_rank();
+
+  // The CTAs of a cluster (JOIN) take one tile together and cut its k-blocks into consecutive ranges; otherwise a CTA
+  // or pair takes whole tiles in steps of the grid.
+  const int tiles = a.tiles_p * a.tiles_q;
+  int kb0 = 0, kb1 = a.kblocks, first_tile = blockIdx.x, step = gridDim.x;
+  if constexpr (JOIN) {
+    first_tile = blockIdx.x / split;
+    step = tiles;
+    const int quads = (a.kblocks + 3) / 4;                 // ranges start on whole scale words
+    kb0 = static_cast<int>(4LL * (static_cast<long long>(quads) * rank / split));
+    kb1 = min(a.kblocks, static_cast<int>(4LL * (static_cast<long long>(quads) * (rank + 1) / split)));
+  }
+  if constexpr (PAIR) {
+    first_tile = blockIdx.x >> 1;
+    step = gridDim.x >> 1;
+  }
+  const int p_off = PAIR ? static_cast<int>(rank) * SG_BP : 0;            // of this CTA within a tile
+  const int q_off = PAIR ? static_cast<int>(rank) * S::Q_ROWS : 0;
+  constexpr int P_TILE = PAIR ? 2 * SG_BP : SG_BP;
+
+  auto load_stage = [&](int s, int kb, int tp, int tq) {
+    uint8_t* dst = smem + s * S::TILE_BYTES;
+    mbar_expect_tx(&full[s], S::TILE_BYTES);
+    tma_load_2d(dst, &tmP, &full[s], kb * 128, tp * P_TILE + p_off);
+    tma_load_2d(dst + S::P_BYTES, &tmQ, &full[s], kb * 128, tq * BQ + q_off);
+  };
+
+  int early = 0;             // k-blocks of the first tile whose loads are issued before the CTA has met
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
-      mbar_init(&full[s], 3);
+      mbar_init(&full[s], PAIR && rank == 0 ? 2 : 1);
       mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < S::SF_SLOTS; ++s) {
+      mbar_init(&sf_full[s], PAIR ? 4 : 2);
+      mbar_init(&sf_empty[s], 1);
     }
     for (int s = 0; s < S::ACCS; ++s) {
       mbar_init(&acc_full[s], 1);
-      mbar_init(&acc_empty[s], SG_EPI_WARPS);
+      mbar_init(&acc_empty[s], PAIR ? 2 * SG_EPI_WARPS : SG_EPI_WARPS);
     }
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tmP);
-    tma_prefetch_desc(&tmQ);
+    grid_dependency_wait();
+    if (first_tile < tiles) {
+      int tp, tq;
+      sg_tile(first_tile, a.tiles_p, a.tiles_q, tp, tq);
+      for (; early < S::STAGES && kb0 + early < kb1; ++early) load_stage(early, kb0 + early, tp, tq);
+    }
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tmem_alloc(tmem_slot, 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before_sync();
   __syncthreads();
+  if constexpr (PAIR) {      // barriers of both CTAs are set up before either arrives on the other's
+    cluster_arrive();
+    cluster_wait();
+  }
+  if constexpr (JOIN)
+    if (split > 1) cluster_arrive();           // waited for before the first push into another CTA
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-
-  // The CTAs of a cluster (JOIN) take one tile together and cut its k-blocks into consecutive ranges; otherwise a CTA
-  // takes whole tiles in steps of the grid.
-  const int tiles = a.tiles_p * a.tiles_q;
-  int kb0 = 0, kb1 = a.kblocks, first_tile = blockIdx.x, step = gridDim.x;
-  uint32_t split = 1, rank = 0;
-  if constexpr (JOIN) {
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(split));
-    rank = cluster_rank();
-    first_tile = blockIdx.x / split;
-    step = tiles;
-    kb0 = static_cast<int>(static_cast<long long>(a.kblocks) * rank / split);
-    kb1 = static_cast<int>(static_cast<long long>(a.kblocks) * (rank + 1) / split);
-  }
+  grid_dependency_wait();
 
   if (warp == 0) {
     if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 0;
+      int s = early == S::STAGES ? 0 : early;
+      uint32_t ph = early == S::STAGES ? 1u : 0u;
       bool ok = true;
+      int skip = early;
       for (int t = first_tile; t < tiles && ok; t += step) {
         int tp, tq;
         sg_tile(t, a.tiles_p, a.tiles_q, tp, tq);
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int kb = kb0 + skip; kb < kb1; ++kb) {
           ok = mbar_wait(&empty[s], ph ^ 1u, abort_flag, status, 1);
           if (!ok) break;
-          uint8_t* dst = smem + s * S::TILE_BYTES;
-          mbar_expect_tx(&full[s], S::TILE_BYTES);
-          tma_load_2d(dst, &tmP, &full[s], kb * 128, tp * SG_BP);
-          tma_load_2d(dst + S::P_BYTES, &tmQ, &full[s], kb * 128, tq * BQ);
+          load_stage(s, kb, tp, tq);
           if (++s == S::STAGES) { s = 0; ph ^= 1u; }
         }
+        skip = 0;
       }
       if (!ok) {                       // a wait gave up: let the copies already issued arrive before the CTA ends
         const uint64_t t0 = globaltimer_ns();
@@ -222,124 +320,185 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constan
       }
     }
   } else if (warp == 2 || warp == 3) {
-    // ------------------------------------------------------------ scale bytes
-    auto run = [&](auto atoms_c, const ScaledOperand& o, int rows_per_tile, bool is_q, int offset) {
+    // ------------------------------------------------------------ scale words
+    // The words of the next four k-blocks are loaded before the present ones are handed over: the fence in front of the
+    // hand-over waits for loads in flight, and once in four k-blocks that is hidden.
+    auto run = [&](auto atoms_c, const ScaledOperand& o, bool is_q, int offset) {
       constexpr int ATOMS = decltype(atoms_c)::value;
-      constexpr int AHEAD = 4;
       int s = 0;
       uint32_t ph = 0;
-      for (int t = first_tile; t < tiles; t += step) {
+      uint32_t w[ATOMS * 4], next[ATOMS * 4];
+      auto row_of = [&](int t) {
         int tp, tq;
         sg_tile(t, a.tiles_p, a.tiles_q, tp, tq);
-        const int row0 = (is_q ? tq : tp) * rows_per_tile;
-        uint32_t w[AHEAD][ATOMS * 4];
+        return is_q ? tq * BQ : tp * P_TILE + p_off;
+      };
+      int row0 = 0;
+      if (first_tile < tiles) {
+        row0 = row_of(first_tile);
+        sg_scale_words<ATOMS>(o, row0, kb0, kb1, next, lane);
+      }
+      for (int t = first_tile; t < tiles; t += step) {
+        for (int kb = kb0; kb < kb1; kb += 4) {
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) sg_load_scales<ATOMS>(o, row0, kb0 + i, kb1, w[i], lane);
-        for (int kb = kb0; kb < kb1; kb += AHEAD) {
+          for (int j = 0; j < ATOMS * 4; ++j) w[j] = next[j];
+          mbar_wait(&sf_empty[s], ph ^ 1u, abort_flag, status, 2);
+          uint8_t* dst = smem + S::SF_OFFSET + s * S::SF_BYTES + offset;
 #pragma unroll
-          for (int i = 0; i < AHEAD; ++i) {
-            if (kb + i < kb1) {
-              mbar_wait(&empty[s], ph ^ 1u, abort_flag, status, 2);
-              uint8_t* dst = smem + S::SF_OFFSET + s * S::SF_BYTES + offset;
-#pragma unroll
-              for (int g = 0; g < ATOMS; ++g) {
-                uint4 v;
-                v.x = w[i][4 * g] * 0x01010101u;
-                v.y = w[i][4 * g + 1] * 0x01010101u;
-                v.z = w[i][4 * g + 2] * 0x01010101u;
-                v.w = w[i][4 * g + 3] * 0x01010101u;
-                *reinterpret_cast<uint4*>(dst + g * 512 + lane * 16) = v;
-              }
-              sg_load_scales<ATOMS>(o, row0, kb + i + AHEAD, kb1, w[i], lane);
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&full[s]);
-              if (++s == S::STAGES) { s = 0; ph ^= 1u; }
-            }
+          for (int g = 0; g < ATOMS; ++g)
+            *reinterpret_cast<uint4*>(dst + g * 512 + lane * 16) = make_uint4(w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (PAIR && rank == 1) mbar_arrive_leader(&sf_full[s]);
+            else mbar_arrive(&sf_full[s]);
           }
+          if (kb + 4 < kb1) {
+            sg_scale_words<ATOMS>(o, row0, kb + 4, kb1, next, lane);
+          } else if (t + step < tiles) {
+            row0 = row_of(t + step);
+            sg_scale_words<ATOMS>(o, row0, kb0, kb1, next, lane);
+          }
+          if (++s == S::SF_SLOTS) { s = 0; ph ^= 1u; }
         }
       }
     };
-    if (warp == 2) run(std::integral_constant<int, 1>{}, a.p, SG_BP, false, 0);
-    else run(std::integral_constant<int, S::Q_ATOMS>{}, a.q, BQ, true, 512);
+    if (warp == 2) run(std::integral_constant<int, 1>{}, a.p, false, 0);
+    else run(std::integral_constant<int, S::Q_ATOMS>{}, a.q, true, 512);
+  } else if (warp == 1 && PAIR && rank == 1) {
+    // ------------------------------------------------------------ this CTA's stages are ready: tell the issuing CTA
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      for (int t = first_tile; t < tiles; t += step)
+        for (int kb = kb0; kb < kb1; ++kb) {
+          mbar_wait(&full[s], ph, abort_flag, status, 6);
+          mbar_arrive_leader(&full[s]);
+          if (++s == S::STAGES) { s = 0; ph ^= 1u; }
+        }
+    }
   } else if (warp == 1) {
     // ------------------------------------------------------------ products
-    constexpr uint32_t idesc = make_idesc_mxf8(BQ);
-    int s = 0, it = 0;
-    uint32_t ph = 0;
+    int s = 0, it = 0, f = 0;
+    uint32_t ph = 0, fph = 0;
     const uint32_t base = smem_u32(smem);
     const uint64_t pd0 = make_smem_desc_sw128(base, 16, 1024);
     const uint64_t qd0 = make_smem_desc_sw128(base + S::P_BYTES, 16, 1024);
     const uint64_t sd0 = make_smem_desc_scales(base + S::SF_OFFSET);
-    for (int t = first_tile; t < tiles; t += step, ++it) {
-      const int as = it % S::ACCS;
-      const uint32_t aph = static_cast<uint32_t>(it / S::ACCS) & 1u;
-      mbar_wait(&acc_empty[as], aph ^ 1u, abort_flag, status, 3);
-      tc_fence_after_sync();
-      const uint32_t d = tmem + static_cast<uint32_t>(as * BQ);
-      for (int kb = kb0; kb < kb1; ++kb) {
-        mbar_wait(&full[s], ph, abort_flag, status, 4);
+    for (int t = first_tile; t < tiles; t += step) {
+      for (int c0 = kb0; c0 < kb1; c0 += a.chunk, ++it) {
+        const int c1 = min(kb1, c0 + a.chunk);
+        const int as = it % S::ACCS;
+        const uint32_t aph = static_cast<uint32_t>(it / S::ACCS) & 1u;
+        mbar_wait(&acc_empty[as], aph ^ 1u, abort_flag, status, 3);
         tc_fence_after_sync();
-        const uint64_t pd = desc_advance(pd0, static_cast<uint32_t>(s * S::TILE_BYTES));
-        const uint64_t qd = desc_advance(qd0, static_cast<uint32_t>(s * S::TILE_BYTES));
-        const uint64_t sd = desc_advance(sd0, static_cast<uint32_t>(s * S::SF_BYTES));
-        const uint32_t sfp = tmem + S::SF_COL + static_cast<uint32_t>(s * 4 * (1 + S::Q_ATOMS));
-        const uint32_t sfq = sfp + 4;
-        if (elect_one()) {
-          tmem_cp_scales(sfp, sd);
+        const uint32_t d = tmem + static_cast<uint32_t>(as * BQ);
+        for (int kb = c0; kb < c1; ++kb) {
+          mbar_wait(&full[s], ph, abort_flag, status, 4);
+          tc_fence_after_sync();
+          const uint64_t pd = desc_advance(pd0, static_cast<uint32_t>(s * S::TILE_BYTES));
+          const uint64_t qd = desc_advance(qd0, static_cast<uint32_t>(s * S::TILE_BYTES));
+          const int byte = kb & 3;
+          const uint32_t sfp = tmem + S::SF_COL + static_cast<uint32_t>(f * S::SF_COLS);
+          const uint32_t sfq = sfp + 4;
+          if (byte == 0) {
+            mbar_wait(&sf_full[f], fph, abort_flag, status, 7);
+            tc_fence_after_sync();
+          }
+          const bool last_of_word = byte == 3 || kb + 1 == kb1;
+          if (elect_one()) {
+            if (byte == 0) {
+              const uint64_t sd = desc_advance(sd0, static_cast<uint32_t>(f * S::SF_BYTES));
+              tmem_cp_scales<PAIR>(sfp, sd);
 #pragma unroll
-          for (int g = 0; g < S::Q_ATOMS; ++g) tmem_cp_scales(sfq + 4 * g, desc_advance(sd, 512 * (1 + g)));
+              for (int g = 0; g < S::Q_ATOMS; ++g) tmem_cp_scales<PAIR>(sfq + 4 * g, desc_advance(sd, 512 * (1 + g)));
+            }
+            const uint32_t idesc = make_idesc_mxf8(P_TILE, BQ, 0) | static_cast<uint32_t>(byte << 4) | (static_cast<uint32_t>(byte) << 29);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)          // 32 codes = 32 bytes of the swizzled row
-            umma_mxf8(d, desc_advance(pd, k * 32), desc_advance(qd, k * 32), idesc, sfp, sfq, (kb > kb0 || k != 0) ? 1u : 0u);
-          umma_commit(&empty[s]);
+            for (int k = 0; k < 4; ++k)          // 32 codes = 32 bytes of the swizzled row
+              umma_mxf8<PAIR>(d, desc_advance(pd, k * 32), desc_advance(qd, k * 32), idesc, sfp, sfq, (kb > c0 || k != 0) ? 1u : 0u);
+            if (last_of_word) sg_commit<PAIR>(&sf_empty[f]);
+            sg_commit<PAIR>(&empty[s]);
+          }
+          __syncwarp();
+          if (last_of_word && ++f == S::SF_SLOTS) { f = 0; fph ^= 1u; }
+          if (++s == S::STAGES) { s = 0; ph ^= 1u; }
         }
+        if (elect_one()) sg_commit<PAIR>(&acc_full[as]);
         __syncwarp();
-        if (++s == S::STAGES) { s = 0; ph ^= 1u; }
       }
-      umma_commit_elect(&acc_full[as]);
     }
   } else {
     // ------------------------------------------------------------ drain
     const int quad = warp & 3, half = (warp - 4) >> 2;
     constexpr int COLS = BQ / 2 < 16 ? 16 : BQ / 2;       // columns per warp (the narrowest tile is drained by four warps)
+    constexpr int GROUP = COLS < 32 ? COLS : 32;
     const bool drains = BQ >= 32 || half == 0;
     const int c_first = BQ >= 32 ? half * COLS : 0;
     int it = 0;
-    for (int t = first_tile; t < tiles; t += step, ++it) {
-      const int as = it % S::ACCS;
-      const uint32_t aph = static_cast<uint32_t>(it / S::ACCS) & 1u;
+    for (int t = first_tile; t < tiles; t += step) {
       int tp, tq;
       sg_tile(t, a.tiles_p, a.tiles_q, tp, tq);
-      mbar_wait(&acc_full[as], aph, abort_flag, status, 5);
-      tc_fence_after_sync();
-      const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(as * BQ + c_first);
-      uint32_t raw[COLS];
-      if (drains) {
-#pragma unroll
-        for (int c = 0; c < COLS; c += 16) tmem_ld_32x16(taddr + c, *reinterpret_cast<uint32_t(*)[16]>(&raw[c]));
-        tmem_ld_wait();
-      }
       float acc[COLS];
 #pragma unroll
-      for (int c = 0; c < COLS; ++c) {
-        asm volatile("" : "+r"(raw[c]));          // no use above the wait
-        acc[c] = __uint_as_float(raw[c]);
-      }
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[as]);
-      if constexpr (JOIN) {
-        // every product of this CTA is done (acc_full), so the tile buffers are free
-        float* dump = reinterpret_cast<float*>(smem);
+      for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
+      for (int c0 = kb0; c0 < kb1; c0 += a.chunk, ++it) {
+        const int as = it % S::ACCS;
+        const uint32_t aph = static_cast<uint32_t>(it / S::ACCS) & 1u;
+        mbar_wait(&acc_full[as], aph, abort_flag, status, 5);
+        tc_fence_after_sync();
+        const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(as * BQ + c_first);
         if (drains) {
 #pragma unroll
-          for (int c = 0; c < COLS; ++c) dump[(c_first + c) * SG_PITCH + quad * 32 + lane] = acc[c];
+          for (int c = 0; c < COLS; c += GROUP) {
+            uint32_t raw[GROUP];
+            if constexpr (GROUP == 32) tmem_ld_32x32(taddr + c, raw);
+            else tmem_ld_32x16(taddr + c, raw);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < GROUP; ++j) {
+              asm volatile("" : "+r"(raw[j]));          // no use above the wait
+              acc[c + j] += __uint_as_float(raw[j]);
+            }
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR && rank == 1) mbar_arrive_leader(&acc_empty[as]);
+          else mbar_arrive(&acc_empty[as]);
+        }
+      }
+      if constexpr (JOIN) {
+        // Column c of the tile is finished by CTA c / slots (SWAP, where few columns may be in use: c % split), at place
+        // c % slots (c / split) of what every CTA sends it.
+        if (SWAP && split == 1) {                        // rows of the output are columns here: lanes along n
+          const int n = tp * SG_BP + quad * 32 + lane;
+          if (drains && n < a.p.rows) {
+            const float b = a.bias != nullptr ? load_typed(a.bias, a.bias_type, n) : 0.f;
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) {
+              const int m = tq * BQ + c_first + c;
+              if (m < a.q.rows) store_typed(a.out, a.out_type, static_cast<long long>(m) * a.ldo + n, acc[c] + b);
+            }
+          }
+          continue;
+        }
+        cluster_wait();                                  // all CTAs of the cluster have started
+        const uint32_t out = smem_u32(smem) + S::OUT_OFFSET + (quad * 32 + lane) * 4;
+        if (drains) {
+          const uint32_t slots = BQ / split;
+#pragma unroll
+          for (int c = 0; c < COLS; ++c) {
+            const uint32_t col = c_first + c;
+            const uint32_t owner = SWAP ? col % split : col / slots, place = SWAP ? col / split : col % slots;
+            st_cluster_f32(cluster_addr(out + (rank * slots + place) * (SG_PITCH * 4), owner), acc[c]);
+          }
         }
       } else {
-        const int row0 = tp * SG_BP + quad * 32;           // rows of the output (p runs along m here)
+        const int row0 = tp * P_TILE + p_off + quad * 32;  // rows of the output (p runs along m here)
         const int col0 = tq * BQ + c_first;
-        uint8_t* stage = smem + S::STAGE_OUT + (warp - 4) * 2048;
+        uint8_t* stage = smem + S::OUT_OFFSET + (warp - 4) * 2048;
         const int rows = a.p.rows - row0, width = a.q.rows;
         if (a.out_type == JB_T_F32) {
 #pragma unroll
@@ -424,43 +583,54 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constan
     }
   }
 
-  if constexpr (JOIN) {
-    // The parts of a tile meet in the shared memory of the cluster; CTA `rank` finishes its share of the output's
-    // columns (SWAP: of the tile's columns, which are rows of the output), always adding the parts in rank order.
-    __syncthreads();
+  if (JOIN && split > 1) {
+    // CTA `rank` finishes its columns of the tile (SWAP: rows of the output), adding the parts in rank order.
     __syncwarp();
-    cluster_arrive_wait();
-    const uint32_t dump = smem_u32(smem);
+    if (warp < 4) cluster_wait();            // the draining warps waited before they pushed
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    const float* parts = reinterpret_cast<const float*>(smem + S::OUT_OFFSET);
+    const int slots = BQ / static_cast<int>(split);
     int tp, tq;
     sg_tile(first_tile, a.tiles_p, a.tiles_q, tp, tq);
     if constexpr (SWAP) {          // p runs along n, q along m: lanes along n
       const int n = tp * SG_BP + (threadIdx.x & 127);
-      const float b = (a.bias != nullptr && n < a.p.rows) ? load_typed(a.bias, a.bias_type, n) : 0.f;
-      const int live = min(BQ, a.q.rows - tq * BQ);
-      for (int c = static_cast<int>(rank) * 3 + (threadIdx.x >> 7); c < live; c += 3 * static_cast<int>(split)) {
-        float v = 0.f;
-        for (uint32_t r = 0; r < split; ++r) v += ld_cluster_f32(dump + (c * SG_PITCH + (threadIdx.x & 127)) * 4, r);
-        if (n < a.p.rows) store_typed(a.out, a.out_type, static_cast<long long>(tq * BQ + c) * a.ldo + n, v + b);
+      if (n < a.p.rows) {
+        const float b = a.bias != nullptr ? load_typed(a.bias, a.bias_type, n) : 0.f;
+        for (int k = threadIdx.x >> 7; k < slots; k += SG_THREADS / 128) {
+          const int m = tq * BQ + k * static_cast<int>(split) + static_cast<int>(rank);
+          if (m >= a.q.rows) break;
+          float v = 0.f;
+          for (int r = 0; r < static_cast<int>(split); ++r) v += parts[(r * slots + k) * SG_PITCH + (threadIdx.x & 127)];
+          store_typed(a.out, a.out_type, static_cast<long long>(m) * a.ldo + n, v + b);
+        }
       }
     } else {                        // lanes along the columns of the tile
-      for (int c0 = 0; c0 < BQ; c0 += 32) {
-        const int c = c0 + lane, n = tq * BQ + c;
-        const float b = (a.bias != nullptr && n < a.q.rows) ? load_typed(a.bias, a.bias_type, n) : 0.f;
-        for (int i = static_cast<int>(rank) * (SG_THREADS / 32) + warp; i < SG_BP; i += static_cast<int>(split) * (SG_THREADS / 32)) {
-          float v = 0.f;
-          for (uint32_t r = 0; r < split; ++r) v += ld_cluster_f32(dump + (c * SG_PITCH + i) * 4, r);
-          const int m = tp * SG_BP + i;
-          if (m < a.p.rows && n < a.q.rows) store_typed(a.out, a.out_type, static_cast<long long>(m) * a.ldo + n, v + b);
+      for (int i = warp; i < SG_BP; i += SG_THREADS / 32) {
+        const int m = tp * SG_BP + i;
+        if (m >= a.p.rows) break;
+        for (int k = lane; k < slots; k += 32) {
+          const int n = tq * BQ + static_cast<int>(rank) * slots + k;
+          if (n >= a.q.rows) break;
+          float v = a.bias != nullptr ? load_typed(a.bias, a.bias_type, n) : 0.f;
+          float sum = 0.f;
+          for (int r = 0; r < static_cast<int>(split); ++r) sum += parts[(r * slots + k) * SG_PITCH + i];
+          store_typed(a.out, a.out_type, static_cast<long long>(m) * a.ldo + n, sum + v);
         }
       }
     }
-    cluster_arrive_wait();          // no CTA leaves while another one reads its shared memory
   }
   tc_fence_before_sync();
   __syncthreads();
+  if constexpr (PAIR) {             // neither CTA leaves while the other's products read its shared memory or arrive on it
+    cluster_arrive();
+    cluster_wait();
+  }
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem, 512);
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    else tmem_dealloc(tmem, 512);
   }
 }
 
@@ -479,30 +649,35 @@ static int make_tmap_codes(CUtensorMap* out, const void* base, long long rows, l
   return r == CUDA_SUCCESS ? 0 : -2;
 }
 
-template <int BQ, bool SWAP, bool JOIN>
+template <int BQ, bool PAIR, bool SWAP, bool JOIN>
 static int launch_scaled_gemm(const void* P, long long pitch_p, const void* Q, long long pitch_q, long long K, ScaledGemmArgs a,
                               int split, int sm_count, int* status, cudaStream_t stream) {
-  using S = SgSmem<BQ, JOIN>;
+  using S = SgSmem<BQ, PAIR, JOIN>;
+  constexpr int P_TILE = PAIR ? 2 * SG_BP : SG_BP;
   CUtensorMap tmP, tmQ;
   if (make_tmap_codes(&tmP, P, a.p.rows, K, pitch_p, SG_BP) != 0) return -2;
-  if (make_tmap_codes(&tmQ, Q, a.q.rows, K, pitch_q, BQ) != 0) return -2;
-  a.tiles_p = (a.p.rows + SG_BP - 1) / SG_BP;
+  if (make_tmap_codes(&tmQ, Q, a.q.rows, K, pitch_q, S::Q_ROWS) != 0) return -2;
+  a.tiles_p = (a.p.rows + P_TILE - 1) / P_TILE;
   a.tiles_q = (a.q.rows + BQ - 1) / BQ;
-  auto kern = scaled_gemm_kernel<BQ, SWAP, JOIN>;
+  auto kern = scaled_gemm_kernel<BQ, PAIR, SWAP, JOIN>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL) != cudaSuccess) return -3;
   const long long tiles = static_cast<long long>(a.tiles_p) * a.tiles_q;
   if (tiles * split > 0x7fffffffLL) return -1;
+  const int cluster = PAIR ? 2 : split;
+  const long long teams = sm_count / (PAIR ? 2 : 1) > 0 ? sm_count / (PAIR ? 2 : 1) : 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(JOIN ? tiles * split : (tiles < sm_count ? tiles : sm_count)));
+  cfg.gridDim = dim3(static_cast<unsigned>(JOIN ? tiles * split : (tiles < teams ? tiles : teams) * cluster));
   cfg.blockDim = dim3(SG_THREADS);
   cfg.dynamicSmemBytes = S::TOTAL;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = split;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = JOIN ? 1 : 0;
+  cfg.numAttrs = JOIN || PAIR ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, tmP, tmQ, a, status) == cudaSuccess ? 0 : -4;
 }
 
@@ -511,34 +686,52 @@ static int launch_scaled_gemm(const void* P, long long pitch_p, const void* Q, l
 extern "C" int jb_scaled_gemm(const JbScaledOperand* a, const JbScaledOperand* b, long long K, void* out, long long ldo,
                               int out_type, const void* bias, int bias_type, int sm_count, int* status, void* stream) {
   using namespace jb;
-  if (a == nullptr || b == nullptr || a->rows < 1 || b->rows < 1 || K < 1 || K > 0x7fffff00LL || sm_count < 1) return -1;
+  if (a == nullptr || b == nullptr || a->rows < 1 || b->rows < 1 || K < 1 || K > 0x7fffff00LL || sm_count < 2) return -1;
   if ((a->pitch & 15) || (b->pitch & 15) || (reinterpret_cast<uintptr_t>(a->codes) & 15) || (reinterpret_cast<uintptr_t>(b->codes) & 15)) return -1;
   if (out_type < 0 || out_type > 2 || bias_type < 0 || bias_type > 2) return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   ScaledGemmArgs g{};
-  const ScaledOperand oa{static_cast<const uint8_t*>(a->scales), a->scale_row, a->scale_k, a->square ? 7 : 0, a->rows};
-  const ScaledOperand ob{static_cast<const uint8_t*>(b->scales), b->scale_row, b->scale_k, b->square ? 7 : 0, b->rows};
+  auto operand = [](const JbScaledOperand* o) {
+    const int words = o->scale_k == 1 && (o->scale_row & 3) == 0 && (reinterpret_cast<uintptr_t>(o->scales) & 3) == 0;
+    return ScaledOperand{static_cast<const uint8_t*>(o->scales), o->scale_row, o->scale_k, o->square ? 7 : 0, o->rows, words};
+  };
+  const ScaledOperand oa = operand(a), ob = operand(b);
   g.out = out; g.ldo = ldo; g.out_type = out_type; g.bias = bias; g.bias_type = bias_type;
   g.kblocks = static_cast<int>((K + 127) / 128);
+  // The tensor cores add into TMEM by truncation, so the error of a sum grows with its length (8192 terms of random sign:
+  // 5e-7 of the result).  fp32 results are drained and added up in registers every 2048 terms; a rounding to 16 bits hides
+  // the rest of them.
+  g.chunk = out_type == JB_T_F32 ? 16 : g.kblocks;
   const int size = out_type == JB_T_F32 ? 4 : 2;
   g.vec_out = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (ldo * size) % 16 == 0;
   const int M = a->rows, N = b->rows;
+#define JB_SG(BQ, PAIR) return launch_scaled_gemm<BQ, PAIR, false, false>(a->codes, a->pitch, b->codes, b->pitch, K, g, 1, sm_count, status, st)
   if (M <= 64) {
-    // few rows: the weight's rows go along the 128 lanes, and several CTAs share a tile's K range until the SMs are busy
     g.p = ob; g.q = oa;
     const int tiles = (N + 127) / 128;
     int split = 1;
-    while (split < 8 && tiles * split * 2 <= sm_count && g.kblocks >= split * 4) split *= 2;
-    if (M <= 16) return launch_scaled_gemm<16, true, true>(b->codes, b->pitch, a->codes, a->pitch, K, g, split, sm_count, status, st);
-    if (M <= 32) return launch_scaled_gemm<32, true, true>(b->codes, b->pitch, a->codes, a->pitch, K, g, split, sm_count, status, st);
-    return launch_scaled_gemm<64, true, true>(b->codes, b->pitch, a->codes, a->pitch, K, g, split, sm_count, status, st);
+    while (split < 8 && tiles * split * 2 <= sm_count && g.kblocks >= split * 8) split *= 2;
+    if (M <= 16) return launch_scaled_gemm<16, false, true, true>(b->codes, b->pitch, a->codes, a->pitch, K, g, split, sm_count, status, st);
+    if (M <= 32) return launch_scaled_gemm<32, false, true, true>(b->codes, b->pitch, a->codes, a->pitch, K, g, split, sm_count, status, st);
+    return launch_scaled_gemm<64, false, true, true>(b->codes, b->pitch, a->codes, a->pitch, K, g, split, sm_count, status, st);
   }
   g.p = oa; g.q = ob;
+  // Tile width.  One k-block costs a CTA about 720 cycles at 128 x 256 and 600 at 128 x 128 (shared memory, which the loads
+  // fill and the products read, is the bound of both), so the wide tile wins unless it leaves a wave of SMs idle:
+  // 4096 x 1024 x 4096 takes 18 us wide and 27 us narrow, 512 x 4096 x 4096 17 us and 15.5 us.
   const long long tiles256 = static_cast<long long>((M + 127) / 128) * ((N + 255) / 256);
-  if (tiles256 >= sm_count) return launch_scaled_gemm<256, false, false>(a->codes, a->pitch, b->codes, b->pitch, K, g, 1, sm_count, status, st);
   const long long tiles128 = static_cast<long long>((M + 127) / 128) * ((N + 127) / 128);
-  int split = 1;
-  while (split < 8 && tiles128 * split * 2 <= sm_count && g.kblocks >= split * 8) split *= 2;
-  if (split > 1) return launch_scaled_gemm<128, false, true>(a->codes, a->pitch, b->codes, b->pitch, K, g, split, sm_count, status, st);
-  return launch_scaled_gemm<128, false, false>(a->codes, a->pitch, b->codes, b->pitch, K, g, 1, sm_count, status, st);
+  const long long waves256 = (tiles256 + sm_count - 1) / sm_count, waves128 = (tiles128 + sm_count - 1) / sm_count;
+  if (waves256 * 720 <= waves128 * 600) {
+    // Pairs load a third less and run longer at higher clocks under the power limit (8192^3: 369 us against 430), but their
+    // hand-overs cost short products a microsecond (4096 x 4096 x 1024: 22.2 us against 21.3).
+    if (g.kblocks >= 16 && tiles256 >= 2LL * sm_count) { JB_SG(256, true); }
+    JB_SG(256, false);
+  }
+  // A tile shared by a cluster costs about 7 us for the meeting of its parts, a k-block 0.31 us: 256 x 1024 x 8192 takes
+  // 24.8 us whole and 16.7 us in four parts, 1024 x 1024 x 4096 15.0 us whole and 19.2 us in two.
+  const int split = tiles128 * 4 <= sm_count && g.kblocks >= 32 ? 4 : tiles128 * 2 <= sm_count && g.kblocks >= 48 ? 2 : 1;
+  if (split > 1) return launch_scaled_gemm<128, false, false, true>(a->codes, a->pitch, b->codes, b->pitch, K, g, split, sm_count, status, st);
+  JB_SG(128, false);
+#undef JB_SG
 }

@@ -148,17 +148,19 @@ struct QuantArgs {
   int square;                // one scale per 128 x 128
 };
 
-// A warp takes 32 rows of one block column, two rows at a time (16 lanes x 8 values); its 32 scale bytes leave together.
+// A warp takes 32 rows of one block column, two rows at a time (16 lanes x 8 values); the scale bytes of the CTA's eight
+// block columns meet in shared memory and leave eight to a row.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
-  const int lane = threadIdx.x & 31, sub = lane & 15;
-  const int kb = blockIdx.y * 8 + (threadIdx.x >> 5);
-  const int col = kb * 128 + sub * 8;
-  if (kb * 128 >= a.cols) return;
+  __shared__ __align__(8) uint8_t bytes[32][8];
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, sub = lane & 15, warp = threadIdx.x >> 5;
+  const int kb0 = blockIdx.y * 8;
+  const int col = (kb0 + warp) * 128 + sub * 8;
   const int live = min(8, max(0, a.cols - col));
+  const long long row0 = static_cast<long long>(blockIdx.x) * 32;
   const T* x = static_cast<const T*>(a.x);
-  for (long long row0 = static_cast<long long>(blockIdx.x) * 32; row0 < a.rows; row0 += static_cast<long long>(gridDim.x) * 32) {
-    uint32_t mine = 127u;
+  if ((kb0 + warp) * 128 < a.cols) {
 #pragma unroll
     for (int i0 = 0; i0 < 16; i0 += 4) {
       if (row0 + 2 * i0 >= a.rows) break;
@@ -170,17 +172,20 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const long long row = row0 + 2 * (i0 + i) + (lane >> 4);
+        const int r = 2 * (i0 + i) + (lane >> 4);
         uint2 q;
         const uint32_t byte = block_of_16_lanes(v[i], q);
-        if (row < a.rows && col < a.pitch) *reinterpret_cast<uint2*>(a.codes + row * a.pitch + col) = q;
-        // row 2 (i0 + i) + h was reduced by lanes 16 h .. 16 h + 15
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, byte, 16);
-        if ((lane >> 1) == i0 + i) mine = (lane & 1) == (lane >> 4) ? byte : other;
+        if (row0 + r < a.rows && col < a.pitch) *reinterpret_cast<uint2*>(a.codes + (row0 + r) * a.pitch + col) = q;
+        if (sub == 0) bytes[r][warp] = static_cast<uint8_t>(byte);
       }
     }
-    const long long row = row0 + lane;
-    if (row < a.rows) a.scales[row * a.scale_row + kb * a.scale_k] = static_cast<uint8_t>(mine);
+  }
+  __syncthreads();
+  // scale_k = 1: a row's bytes of this CTA are neighbours
+  const int n = min(8, (a.cols + 127) / 128 - kb0);
+  {
+    const int r = threadIdx.x >> 3, k = threadIdx.x & 7;
+    if (row0 + r < a.rows && k < n) a.scales[(row0 + r) * a.scale_row + (kb0 + k) * a.scale_k] = bytes[r][k];
   }
 }
 
@@ -206,6 +211,7 @@ struct TileShared {
 template <typename T, bool VEC, bool NORM>
 __global__ void __launch_bounds__(512, 2) quant_tile_kernel(const QuantArgs a) {
   __shared__ TileShared sh;
+  grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tile_r = blockIdx.x, tile_c = blockIdx.y;
   const long long row0 = static_cast<long long>(tile_r) * 128 + warp * 8;
@@ -353,6 +359,7 @@ __global__ void __launch_bounds__(512, 2) quant_tile_kernel(const QuantArgs a) {
 // out[c] = sum over the rows of part [P, C], 32 columns a CTA; the order of the additions is fixed.
 __global__ void __launch_bounds__(1024) column_sum_kernel(const float* part, int P, int C, void* out, int out_type) {
   __shared__ float sums[32][33];
+  grid_dependency_wait();
   const int c = blockIdx.x * 32 + threadIdx.x;
   float t = 0.f;
   if (c < C)
@@ -464,6 +471,7 @@ __device__ __forceinline__ double row_sum(double v, double* shared) {
 template <typename T, int NV, bool VEC, bool WARP, bool CODES, int MOST>
 __global__ void __launch_bounds__(MOST) rms_fwd_kernel(const RmsArgs a) {
   __shared__ double shared[32];
+  grid_dependency_wait();
   const int G = WARP ? 32 : blockDim.x;                          // threads of a row
   const int g = WARP ? (threadIdx.x & 31) : threadIdx.x;
   const long long row = WARP ? static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
@@ -538,6 +546,7 @@ struct RmsBwdArgs {
 template <typename T, typename TG, int NV, bool VEC, bool WARP, int MOST>
 __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) rms_bwd_kernel(const RmsBwdArgs a) {
   __shared__ double shared[2][32];
+  grid_dependency_wait();
   const int G = WARP ? 32 : blockDim.x;
   const int g = WARP ? (threadIdx.x & 31) : threadIdx.x;
   const long long first = WARP ? static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
@@ -606,6 +615,22 @@ __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) rms_bwd_kernel(cons
 }
 
 // ---------------------------------------------------------------- dispatch
+// Launch that may begin while earlier work of the stream still runs: every kernel here calls grid_dependency_wait() before
+// it touches memory, so only its launch and set-up overlap (about 2 us a launch in a chain of short kernels).
+template <typename Kernel, typename Args, typename... More>
+static cudaError_t launch_chained(Kernel kernel, dim3 grid, dim3 block, cudaStream_t stream, const Args& first, More... more) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, first, more...);
+}
+
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Threads of a CTA that takes one row, `held` values each.
@@ -617,11 +642,11 @@ template <typename T, bool VEC, bool CODES>
 static int launch_rms_fwd(const RmsArgs& a, int sm_count, cudaStream_t st) {
   const int warps = (a.rows + 7) / 8;
   if (a.rows < sm_count && a.cols > 256 && a.cols <= 8192)
-    rms_fwd_kernel<T, 1, VEC, false, CODES, 1024><<<a.rows, rms_threads(a.cols, 8), 0, st>>>(a);
-  else if (a.cols <= 512) rms_fwd_kernel<T, 2, VEC, true, CODES, 256><<<warps, 256, 0, st>>>(a);
-  else if (a.cols <= 1024) rms_fwd_kernel<T, 4, VEC, true, CODES, 256><<<warps, 256, 0, st>>>(a);
-  else if (a.cols <= 16384) rms_fwd_kernel<T, 4, VEC, false, CODES, 512><<<a.rows, rms_threads(a.cols, 32), 0, st>>>(a);
-  else rms_fwd_kernel<T, 4, VEC, false, CODES, 1024><<<a.rows, rms_threads(a.cols, 32), 0, st>>>(a);
+    launch_chained(rms_fwd_kernel<T, 1, VEC, false, CODES, 1024>, dim3(a.rows), dim3(rms_threads(a.cols, 8)), st, a);
+  else if (a.cols <= 512) launch_chained(rms_fwd_kernel<T, 2, VEC, true, CODES, 256>, dim3(warps), dim3(256), st, a);
+  else if (a.cols <= 1024) launch_chained(rms_fwd_kernel<T, 4, VEC, true, CODES, 256>, dim3(warps), dim3(256), st, a);
+  else if (a.cols <= 16384) launch_chained(rms_fwd_kernel<T, 4, VEC, false, CODES, 512>, dim3(a.rows), dim3(rms_threads(a.cols, 32)), st, a);
+  else launch_chained(rms_fwd_kernel<T, 4, VEC, false, CODES, 1024>, dim3(a.rows), dim3(rms_threads(a.cols, 32)), st, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
@@ -642,11 +667,11 @@ static inline int rms_bwd_ctas(int rows, int cols, int sm_count) {
 template <typename T, typename TG, bool VEC>
 static int launch_rms_bwd(const RmsBwdArgs& a, int sm_count, cudaStream_t st) {
   const int grid = rms_bwd_ctas(a.rows, a.cols, sm_count), threads = rms_bwd_threads(a.cols);
-  if (rms_bwd_by_warp(a.cols)) rms_bwd_kernel<T, TG, 2, VEC, true, 256><<<grid, threads, 0, st>>>(a);
-  else if (threads <= 256 && a.cols <= 8192) rms_bwd_kernel<T, TG, 2, VEC, false, 256><<<grid, threads, 0, st>>>(a);
-  else if (a.cols <= 8192) rms_bwd_kernel<T, TG, 2, VEC, false, 512><<<grid, threads, 0, st>>>(a);
-  else if (a.cols <= 16384) rms_bwd_kernel<T, TG, 4, VEC, false, 512><<<grid, threads, 0, st>>>(a);
-  else rms_bwd_kernel<T, TG, 4, VEC, false, 1024><<<grid, threads, 0, st>>>(a);
+  if (rms_bwd_by_warp(a.cols)) launch_chained(rms_bwd_kernel<T, TG, 2, VEC, true, 256>, dim3(grid), dim3(threads), st, a);
+  else if (threads <= 256 && a.cols <= 8192) launch_chained(rms_bwd_kernel<T, TG, 2, VEC, false, 256>, dim3(grid), dim3(threads), st, a);
+  else if (a.cols <= 8192) launch_chained(rms_bwd_kernel<T, TG, 2, VEC, false, 512>, dim3(grid), dim3(threads), st, a);
+  else if (a.cols <= 16384) launch_chained(rms_bwd_kernel<T, TG, 4, VEC, false, 512>, dim3(grid), dim3(threads), st, a);
+  else launch_chained(rms_bwd_kernel<T, TG, 4, VEC, false, 1024>, dim3(grid), dim3(threads), st, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
@@ -659,18 +684,18 @@ static int launch_quant(const QuantArgs& a, bool tiles, cudaStream_t st) {
     if (kblocks > 65535) return -1;
     const dim3 grid(rblocks, kblocks);
     if (a.rstd != nullptr) {
-      if (vec) quant_tile_kernel<T, true, true><<<grid, 512, 0, st>>>(a);
-      else quant_tile_kernel<T, false, true><<<grid, 512, 0, st>>>(a);
+      if (vec) launch_chained(quant_tile_kernel<T, true, true>, dim3(grid), dim3(512), st, a);
+      else launch_chained(quant_tile_kernel<T, false, true>, dim3(grid), dim3(512), st, a);
     } else {
-      if (vec) quant_tile_kernel<T, true, false><<<grid, 512, 0, st>>>(a);
-      else quant_tile_kernel<T, false, false><<<grid, 512, 0, st>>>(a);
+      if (vec) launch_chained(quant_tile_kernel<T, true, false>, dim3(grid), dim3(512), st, a);
+      else launch_chained(quant_tile_kernel<T, false, false>, dim3(grid), dim3(512), st, a);
     }
   } else {
     const bool vec = a.cols % 8 == 0 && (a.ldx * size) % 16 == 0 && aligned16(a.x);
     if ((kblocks + 7) / 8 > 65535) return -1;
     const dim3 grid((a.rows + 31) / 32, (kblocks + 7) / 8);
-    if (vec) quant_rows_kernel<T, true><<<grid, 256, 0, st>>>(a);
-    else quant_rows_kernel<T, false><<<grid, 256, 0, st>>>(a);
+    if (vec) launch_chained(quant_rows_kernel<T, true>, dim3(grid), dim3(256), st, a);
+    else launch_chained(quant_rows_kernel<T, false>, dim3(grid), dim3(256), st, a);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
@@ -703,8 +728,7 @@ extern "C" int jb_quantize(const JbQuant* q, void* stream) {
 
 extern "C" int jb_column_sum(const float* part, int P, int C, void* out, int out_type, void* stream) {
   if (P < 1 || C < 1) return -1;
-  jb::column_sum_kernel<<<(C + 31) / 32, dim3(32, 32), 0, static_cast<cudaStream_t>(stream)>>>(part, P, C, out, out_type);
-  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+  return jb::launch_chained(jb::column_sum_kernel, dim3((C + 31) / 32), dim3(32, 32), static_cast<cudaStream_t>(stream), part, P, C, out, out_type) == cudaSuccess ? 0 : -4;
 }
 
 // Longest row that the kernels keep in registers.

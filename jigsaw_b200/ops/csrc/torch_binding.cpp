@@ -80,16 +80,21 @@ struct Codes {
   Tensor codes, scales;
   int64_t rows = 0, cols = 0, scale_row = 0, scale_k = 0;
   bool square = false;
-  bool turned = false;       // `scales` is stored blocks first
+  bool turned = false;       // `scales` are those of the transpose
 
   JbScaledOperand operand() const {
     return {codes.data_ptr(), codes.size(1), scales.data_ptr(), scale_row, scale_k, static_cast<int>(rows), square ? 1 : 0};
   }
   // The public forms: [rows, cols] and [scale rows, blocks].
   Tensor code_view() const { return codes.size(1) == cols ? codes : codes.narrow(1, 0, cols); }
-  Tensor scale_view() const { return turned ? scales.t() : scales; }
+  Tensor scale_view() const {
+    const int64_t blocks = ((turned ? rows : cols) + 127) / 128;
+    const Tensor s = scales.size(1) == blocks ? scales : scales.narrow(1, 0, blocks);
+    return turned ? s.t() : s;
+  }
 };
-// Scales per row are stored block by block, rows contiguous: a warp of the product reads 32 rows in one request.
+// The scales of a row start on a whole word: the product reads those of four blocks at once.
+int64_t words_of(int64_t blocks) { return (blocks + 3) / 4 * 4; }
 Codes new_codes(int64_t rows, int64_t cols, const Tensor& like) {
   Codes q;
   q.rows = rows;
@@ -98,10 +103,9 @@ Codes new_codes(int64_t rows, int64_t cols, const Tensor& like) {
   return q;
 }
 void new_row_scales(Codes& q) {
-  q.scales = empty({(q.cols + 127) / 128, q.rows}, SCALES, q.codes);
-  q.scale_row = 1;
-  q.scale_k = q.rows;
-  q.turned = true;
+  q.scales = empty({q.rows, words_of((q.cols + 127) / 128)}, SCALES, q.codes);
+  q.scale_row = q.scales.size(1);
+  q.scale_k = 1;
 }
 
 struct Quantized {
@@ -126,9 +130,9 @@ Quantized quantize(const Tensor& input, bool square, bool want_rows, bool want_c
   Quantized out;
   Tensor shared;
   if (square) {
-    shared = empty({rb, cb}, SCALES, x.t);
+    shared = empty({rb, words_of(cb)}, SCALES, x.t);
     q.scales = shared.data_ptr();
-    q.scale_row = cb;
+    q.scale_row = shared.size(1);
     q.scale_k = 1;
   }
   if (want_rows) {
@@ -137,7 +141,7 @@ Quantized quantize(const Tensor& input, bool square, bool want_rows, bool want_c
     q.pitch = c.codes.size(1);
     if (square) {
       c.scales = shared;
-      c.scale_row = cb;
+      c.scale_row = shared.size(1);
       c.scale_k = 1;
       c.square = true;
     } else {
@@ -155,7 +159,7 @@ Quantized quantize(const Tensor& input, bool square, bool want_rows, bool want_c
     if (square) {
       c.scales = shared;
       c.scale_row = 1;
-      c.scale_k = cb;
+      c.scale_k = shared.size(1);
       c.square = c.turned = true;
     } else {
       new_row_scales(c);
@@ -327,9 +331,9 @@ Codes saved_codes(const Tensor& codes, const Tensor& scales, int64_t rows, int64
   c.scales = scales;
   c.rows = rows;
   c.cols = cols;
-  c.square = square;
-  c.scale_row = 1;
-  c.scale_k = scales.size(1);
+  c.square = c.turned = square;
+  c.scale_row = square ? 1 : scales.size(1);
+  c.scale_k = square ? scales.size(1) : 1;
   return c;
 }
 std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
@@ -551,7 +555,7 @@ py::tuple py_rms_quantize(const Tensor& x, const Optional& gain, double eps, con
                           bool want_rstd) {
   const Normed n = rms_forward(x, opt(gain), eps, opt(residual), -1, true, want_rstd);
   Tensor codes = n.codes->code_view(), scales = n.codes->scale_view();
-  if (x.dim() != 2) {
+  if (x.dim() != 2) {              // splitting the rows of a strided matrix is a view
     codes = codes.view(x.sizes());
     scales = scales.view(with_last(x, scales.size(1)));
   }
