@@ -25,7 +25,7 @@ from typing import Any, Literal
 import torch
 from torch import nn
 
-from .modules import activation, attention, convolution, linear, normalization, roll
+from .modules import activation, attention, convolution, linear, normalization, roll, scaled
 
 __all__ = [
     "ConversionPlan",
@@ -47,6 +47,7 @@ mapped_modules: dict[type[nn.Module], Any] = {
     roll.Roll: roll.DistributedRoll,
     nn.LayerNorm: normalization.DistributedLayerNorm,
     nn.GroupNorm: normalization.DistributedGroupNorm,
+    nn.RMSNorm: scaled.DistributedRMSNorm,
     nn.Softmax: activation.DistributedSoftmax,
     linear.MatMulXWT: linear.DistributedMatMulXWT,
     linear.MatMulXW: linear.DistributedMatMulXW,

@@ -8,7 +8,7 @@ Every tensor stays sharded from input to loss::
     patch embedding   DistributedConv2d, kernel == stride (no halo)
     attention         DistributedAttention: ring or Ulysses over "row", heads over "col"
     MLP               DistributedLinear, weights split over both axes
-    norms             DistributedLayerNorm, statistics reduced over "col"
+    norms             DistributedLayerNorm or DistributedRMSNorm, statistics reduced over "col"
     output            image-to-image (DistributedConvTranspose2d patch recovery, residual)
                       or classification (token mean over "row", class logits over "col")
 
@@ -37,6 +37,8 @@ from ..modules import (
     DistributedConvTranspose2d,
     DistributedLayerNorm,
     DistributedLinear,
+    DistributedRMSNorm,
+    LinearConfig,
     RingAttentionConfig,
 )
 from ..modules.attention import SaveBackward, SendForward
@@ -57,6 +59,8 @@ class ViTConfig:
     sequence_parallel: str = "ring"     # "ring" | "ulysses"
     attn_backend: str = "sdpa"
     dtype: torch.dtype = torch.float32
+    norm: str = "layer"                 # "layer" | "rms" (root-mean-square norms, residual added in the norm's kernel)
+    linear_precision: str = "native"    # "native" | "fp8": the products of the MLP in 8 bits with block scales
     recompute_blocks: bool = False      # activation checkpointing: keep only each block's input, recompute in backward
 
 
@@ -76,14 +80,19 @@ def sincos_position(dim: int, h_idx: torch.Tensor, w_idx: torch.Tensor) -> torch
     return torch.cat((grid_h, grid_w), dim=-1)
 
 
+def _norm(cfg: ViTConfig, mesh: Mesh, device: torch.device) -> nn.Module:
+    kind = DistributedRMSNorm if cfg.norm == "rms" else DistributedLayerNorm
+    return kind(cfg.dim, None, device, mesh["row"], mesh["col"], dtype=cfg.dtype)
+
+
 class ViTBlock(nn.Module):
     """Pre-norm block: ``x + attention(norm(x))`` then ``x + mlp(norm(x))``."""
 
     def __init__(self, cfg: ViTConfig, mesh: Mesh, device: torch.device) -> None:
         super().__init__()
         row, col, model = mesh["row"], mesh["col"], mesh["model"]
-        self.norm1 = DistributedLayerNorm(cfg.dim, None, device, row, col, dtype=cfg.dtype)
-        self.norm2 = DistributedLayerNorm(cfg.dim, None, device, row, col, dtype=cfg.dtype)
+        self.norm1 = _norm(cfg, mesh, device)
+        self.norm2 = _norm(cfg, mesh, device)
         ring = cfg.sequence_parallel == "ring" and row.size() > 1
         ulysses = cfg.sequence_parallel == "ulysses" and row.size() > 1
         ring_cfg = None
@@ -96,11 +105,15 @@ class ViTBlock(nn.Module):
             ulysses=ulysses, attn_backend=cfg.attn_backend, dtype=cfg.dtype, config=ring_cfg,
         )
         hidden = cfg.mlp_ratio * cfg.dim
-        self.fc1 = DistributedLinear(cfg.dim, hidden, device, model, row, col, dtype=cfg.dtype)
+        linear = LinearConfig(model, linear_layer=True, device=device, precision=cfg.linear_precision)
+        self.fc1 = DistributedLinear(cfg.dim, hidden, device, model, row, col, config=linear, dtype=cfg.dtype)
         self.act = nn.GELU()
-        self.fc2 = DistributedLinear(hidden, cfg.dim, device, model, row, col, dtype=cfg.dtype)
+        self.fc2 = DistributedLinear(hidden, cfg.dim, device, model, row, col, config=linear, dtype=cfg.dtype)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if isinstance(self.norm2, DistributedRMSNorm):          # the sum leaves the norm's kernel with the first MLP product
+            h, x = self.norm2.forward_linear(self.attn(self.norm1(x)), self.fc1, residual=x)
+            return x + self.fc2(self.act(h))
         x = x + self.attn(self.norm1(x))
         return x + self.fc2(self.act(self.fc1(self.norm2(x))))
 
@@ -112,6 +125,8 @@ class ViT(nn.Module):
         device = torch.device(device)
         if cfg.sequence_parallel not in ("ring", "ulysses"):
             raise ValueError(f"sequence_parallel must be 'ring' or 'ulysses', got {cfg.sequence_parallel!r}")
+        if cfg.norm not in ("layer", "rms"):
+            raise ValueError(f"norm must be 'layer' or 'rms', got {cfg.norm!r}")
         if cfg.dim % 4:
             raise ValueError("dim must be a multiple of 4 for the sin/cos position embedding")
         row, col = mesh["row"], mesh["col"]
@@ -123,7 +138,7 @@ class ViT(nn.Module):
                      dtype=cfg.dtype)
         self.embed = DistributedConv2d(cfg.in_channels, cfg.dim, **patch)
         self.blocks = nn.ModuleList(ViTBlock(cfg, mesh, device) for _ in range(cfg.depth))
-        self.norm = DistributedLayerNorm(cfg.dim, None, device, row, col, dtype=cfg.dtype)
+        self.norm = _norm(cfg, mesh, device)
         if cfg.num_classes is None:
             self.recover = DistributedConvTranspose2d(cfg.dim, cfg.in_channels, **patch)
             self.head = None

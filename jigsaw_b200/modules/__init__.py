@@ -9,6 +9,9 @@ importable from here, and ``CommOp`` names the transport of the neighbour exchan
 axis, a loss, a metric, a norm's spatial cut, a softmax and the block products ``None`` means "not cut"), converts from and to its ``torch.nn`` counterpart, and can be moved between meshes with
 ``reshard_parameters``.
 
+``scaled`` holds the 8-bit token path (root-mean-square norm, block quantisation, 8-bit matrix products), which the
+reference does not have.
+
 Reference parity: jigsaw/modules/__init__.py:61-112.
 """
 
@@ -51,7 +54,12 @@ from .normalization import DistributedGroupNorm, DistributedLayerNorm
 from .roll import DistributedRoll, Roll, RollConfig
 
 # everything imported above is public: the ten sub-packages, the layer and configuration classes, and CommOp
-__all__ = sorted(name for name in dir() if not name.startswith("_") and name != "set_module")
+# (``scaled``, which ``functional`` has loaded, lists its names itself)
+__all__ = sorted(name for name in dir() if not name.startswith("_") and name not in ("scaled", "set_module"))
 
 set_module(globals(), [name for name in __all__ if name != "CommOp"])
 CommOp.__module__ = __name__
+
+# beyond the reference's names: the 8-bit token path, listed by its own module
+from . import scaled  # noqa: E402, F401
+from .scaled import DistributedRMSNorm  # noqa: E402, F401

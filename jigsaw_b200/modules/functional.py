@@ -14,17 +14,16 @@
 ``distributed_confusion_matrix``                    class-by-class counts over all tiles
 ``confusion_to_metrics``                            accuracy, IoU, Dice, precision, recall from the counts
 ``distributed_permute``                             ``permute`` that also moves the cut from one axis to another
-``distributed_rms_norm``                            root-mean-square norm along a cut axis, with the residual's addition
-``quantize_blockwise``                              8-bit codes with power-of-two block scales (``BlockScaled``)
-``scaled_matmul`` / ``scaled_linear``               product of two ``BlockScaled``; differentiable 8-bit linear layer
-``rms_norm_quantize`` / ``rms_norm_linear``         norm with an 8-bit output; norm fused in front of the 8-bit linear layer
 ==================================================  ==============================================================
+
+The functions of the 8-bit token path (``distributed_rms_norm``, ``quantize_blockwise``, ``scaled_matmul``,
+``scaled_linear``, ``rms_norm_quantize``, ``rms_norm_linear``, and the class ``BlockScaled``) are importable from here
+too; ``jigsaw_b200.modules.scaled`` documents and lists them.
 
 Reference parity: jigsaw/modules/functional.py:19-37.
 """
 
 from .activation import distributed_argmax, distributed_log_softmax
-from .linear import BlockScaled, quantize_blockwise, scaled_linear, scaled_matmul
 from .loss import (
     distributed_binary_cross_entropy,
     distributed_binary_cross_entropy_with_logits,
@@ -36,11 +35,18 @@ from .loss import (
     redundant_all_reduce,
 )
 from .metrics import confusion_to_metrics, distributed_confusion_matrix
-from .normalization import distributed_rms_norm, rms_norm_linear, rms_norm_quantize
 from .permute import distributed_permute
+from .scaled import (  # noqa: F401
+    BlockScaled,
+    distributed_rms_norm,
+    quantize_blockwise,
+    rms_norm_linear,
+    rms_norm_quantize,
+    scaled_linear,
+    scaled_matmul,
+)
 
 __all__ = [
-    "BlockScaled",
     "confusion_to_metrics",
     "distributed_argmax",
     "distributed_binary_cross_entropy",
@@ -52,12 +58,6 @@ __all__ = [
     "distributed_mse_loss",
     "distributed_nll_loss",
     "distributed_permute",
-    "distributed_rms_norm",
     "distributed_smooth_l1_loss",
-    "quantize_blockwise",
     "redundant_all_reduce",
-    "rms_norm_linear",
-    "rms_norm_quantize",
-    "scaled_linear",
-    "scaled_matmul",
 ]

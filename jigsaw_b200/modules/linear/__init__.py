@@ -22,10 +22,8 @@ from ._linear import (
     MatMulXW,
     MatMulXWT,
 )
-from ._scaled import BlockScaled, quantize_blockwise, scaled_linear, scaled_matmul
 
 __all__ = [
-    "BlockScaled",
     "DistributedLinear",
     "DistributedMatMulXTW",
     "DistributedMatMulXW",
@@ -34,9 +32,6 @@ __all__ = [
     "MatMulXTW",
     "MatMulXW",
     "MatMulXWT",
-    "quantize_blockwise",
-    "scaled_linear",
-    "scaled_matmul",
 ]
 
 set_module(globals(), __all__)

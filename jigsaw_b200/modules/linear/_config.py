@@ -36,10 +36,18 @@ class LinearConfig:
         linear_layer: bool = True,
         device: torch.device | str = "cuda",
         comm: CommOp | str = "auto",
+        precision: str = "native",
     ) -> None:
+        """``precision``: "native" multiplies in the autocast type or that of the operands; "fp8" quantises the operands of a
+        linear layer's three products to 8 bits with block scales (``modules.scaled.scaled_linear``)."""
+        if precision not in ("native", "fp8"):
+            raise ValueError(f"precision must be 'native' or 'fp8', got {precision!r}")
+        if precision == "fp8" and not linear_layer:
+            raise ValueError("precision='fp8' is for linear layers; products of two activations run in the native precision")
         self.device = torch.device(device)
         self.comm = resolve_comm_op(comm, self.device)
         self.linear_layer = linear_layer
+        self.precision = precision
         self.model_size = 1 if model_group is None else model_group.size()          # None: a single process
         self._layer_key = {"model group size": self.model_size, "linear_layer": linear_layer}
         self.vmapped = False

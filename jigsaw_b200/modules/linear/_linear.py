@@ -33,9 +33,12 @@ from ..._core.placement import check_divisible, gather_dim
 from ..._core.shard_repr import shard_repr
 from ._config import LinearConfig, default_grid
 from ._functional import block_matmul, fetch_region
+from ._scaled import scaled_linear
 
 
-def _local_linear(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None) -> torch.Tensor:
+def _local_linear(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, precision: str = "native") -> torch.Tensor:
+    if precision == "fp8":
+        return scaled_linear(x, w, b)
     if x.is_cuda:
         from ...ops import linear_fused
 
@@ -131,7 +134,8 @@ class DistributedLinear(torch.nn.Module):
         """The ``(out / C, in)`` rows of the global weight that make this rank's output block, fetched block by
         block from their owners (in the compute dtype): ``R / C`` row blocks times ``C`` column blocks, i.e.
         ``out * in / C`` elements in flight, never the whole matrix."""
-        (w,) = cast_to_autocast_dtype(w)
+        if self.config.precision != "fp8":             # the 8-bit products quantise the weight as it is stored
+            (w,) = cast_to_autocast_dtype(w)
         C, n = self.col_split, self.out_dim // self.col_split
         k = w.shape[1]
         if self.row_split > 1:
@@ -144,7 +148,7 @@ class DistributedLinear(torch.nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         w, b = parallel.sync_grad(self.weight, self.bias)
         w_j = self._out_block_weight(w)                                     # (N/C, K)
-        if x.is_cuda and self.col_split > 1:
+        if x.is_cuda and self.col_split > 1 and self.config.precision != "fp8":
             from ...ops import linear_fused
 
             # all-gather of x fused into the GEMM: the kernel reads the peers' blocks itself
@@ -152,19 +156,19 @@ class DistributedLinear(torch.nn.Module):
             if out is not None:
                 return out
         x_full = all_gather_cat(x, self.col_group, -1)                     # (.., M/R, K)
-        return _local_linear(x_full, w_j, b)
+        return _local_linear(x_full, w_j, b, self.config.precision)
 
     # ------------------------------------------------------------------ conversion
     @classmethod
     def convert_to_jigsaw(
         cls, model: torch.nn.Linear, process_mesh_dict: dict, device: torch.device | str, row_kw: str = "row",
-        col_kw: str = "col", model_kw: str = "model", comm: str = "auto", **kwargs: Any,
+        col_kw: str = "col", model_kw: str = "model", comm: str = "auto", precision: str = "native", **kwargs: Any,
     ) -> "DistributedLinear":
         mg = process_mesh_dict[model_kw]
         layer = cls(
             model.in_features, model.out_features, device, mg, process_mesh_dict[row_kw], process_mesh_dict[col_kw],
             bias=model.bias is not None, dtype=model.weight.dtype,
-            config=LinearConfig(mg, linear_layer=True, device=device, comm=comm),
+            config=LinearConfig(mg, linear_layer=True, device=device, comm=comm, precision=precision),
         )
         layer._load_global(model.weight.data, None if model.bias is None else model.bias.data)
         return layer
@@ -225,7 +229,8 @@ class DistributedLinear(torch.nn.Module):
         w, b = self.merge_weights(from_process_mesh, pm_row_key, pm_col_key, pm_model_key)
         self._bind_groups(new_model, to_process_mesh[pm_row_key], to_process_mesh[pm_col_key])
         self._model_is_col = col_only
-        self.config = LinearConfig(new_model, linear_layer=True, device=self.device, comm=self.config.comm)
+        self.config = LinearConfig(new_model, linear_layer=True, device=self.device, comm=self.config.comm,
+                                   precision=self.config.precision)
         self.weight = torch.nn.Parameter(torch.empty(0, device=self.device, dtype=w.dtype))
         if self.bias is not None:
             self.bias = torch.nn.Parameter(torch.empty(0, device=self.device, dtype=w.dtype))
@@ -246,6 +251,7 @@ class DistributedLinear(torch.nn.Module):
         return (
             f"in_features={self.in_dim}, out_features={self.out_dim}, bias={self.bias is not None}, "
             + shard_repr(row=self.row_split, col=self.col_group)
+            + (", precision=fp8" if self.config.precision == "fp8" else "")
         )
 
 

@@ -12,8 +12,7 @@ Reference parity: jigsaw/modules/normalization/__init__.py (two public names).
 from ..._core.public import set_module
 from ._group_norm import DistributedGroupNorm
 from ._layer_norm import DistributedLayerNorm
-from ._rms_functional import distributed_rms_norm, rms_norm_linear, rms_norm_quantize
 
-__all__ = ["DistributedGroupNorm", "DistributedLayerNorm", "distributed_rms_norm", "rms_norm_linear", "rms_norm_quantize"]
+__all__ = ["DistributedGroupNorm", "DistributedLayerNorm"]
 
 set_module(globals(), __all__)
