@@ -20,9 +20,12 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ..._core.autocast import autocast_dtype
+from ...ops import scaled_fused
 
 BLOCK = 128
 ROW, SQUARE = (1, BLOCK), (BLOCK, BLOCK)
+_HALF = (torch.float32, torch.bfloat16, torch.float16)
+_batched = torch._C._functorch.is_batchedtensor
 
 
 @dataclass(frozen=True, eq=False)
@@ -56,7 +59,19 @@ class BlockScaled:
         return _values(self.codes, self.scales, self.block).to(dtype)
 
 
+def _made(codes: torch.Tensor, scales: torch.Tensor, block: tuple[int, int]) -> BlockScaled:
+    """A ``BlockScaled`` of parts that belong together (no checks)."""
+    q = object.__new__(BlockScaled)
+    put = object.__setattr__
+    put(q, "codes", codes)
+    put(q, "scales", scales)
+    put(q, "block", block)
+    return q
+
+
 def _check_block(block: tuple[int, int]) -> tuple[int, int]:
+    if block == ROW or block == SQUARE:
+        return block
     block = tuple(block)
     if block not in (ROW, SQUARE):
         raise ValueError(f"blocks are (1, 128) or (128, 128), got {block}")
@@ -106,12 +121,11 @@ def _quantize_2d(x: torch.Tensor, block: tuple[int, int], rows: bool = True, col
     """``x [R, C]`` (times ``rstd`` per row and ``gain`` per column) in blocks along its rows, its transpose in blocks along the
     columns of ``x``, and the column sums of the values."""
     if x.is_cuda:
-        from ...ops import scaled_fused
-
-        out = scaled_fused.maybe_fused_quantize(x, block == SQUARE, rows, cols, rstd, gain, colsum)
+        out = scaled_fused.quantize_both(x, block == SQUARE, rows, cols, rstd, gain, colsum)
         if out is not None:
             c, s, ct, st, sums = out
-            return (None if c is None else BlockScaled(c, s, block)), (None if ct is None else BlockScaled(ct, st, block)), sums
+            return (None if c is None else _made(c, s, block)), (None if ct is None else _made(ct, st, block)), sums
+        scaled_fused.declined("quantize", "outside the coverage of the kernel")
     v = x
     if rstd is not None:
         v = v.float() * rstd[:, None]
@@ -126,11 +140,10 @@ def _quantize_2d(x: torch.Tensor, block: tuple[int, int], rows: bool = True, col
 def _product(a: BlockScaled, b: BlockScaled, bias: torch.Tensor | None, out_dtype: torch.dtype) -> torch.Tensor:
     """``a [..., K] b [N, K]^T + bias``."""
     if a.codes.is_cuda:
-        from ...ops import scaled_fused
-
-        out = scaled_fused.maybe_fused_scaled_matmul(a, b, bias, out_dtype)
+        out = scaled_fused.scaled_matmul(a, b, bias, out_dtype)
         if out is not None:
             return out
+        scaled_fused.declined("scaled_matmul", "outside the coverage of the kernel")
     y = a.dequantize() @ b.dequantize().t()
     if bias is not None:
         y = y + bias.float()
@@ -139,8 +152,9 @@ def _product(a: BlockScaled, b: BlockScaled, bias: torch.Tensor | None, out_dtyp
 
 # ----------------------------------------------------------------------------- public functions
 def _refuse_vmap(name: str, *tensors: Any) -> None:
-    if any(isinstance(t, torch.Tensor) and torch._C._functorch.is_batchedtensor(t) for t in tensors):
-        raise NotImplementedError(f"{name} has no batching rule for torch.vmap; give it the members as leading dimensions")
+    for t in tensors:
+        if t is not None and _batched(t):
+            raise NotImplementedError(f"{name} has no batching rule for torch.vmap; give it the members as leading dimensions")
 
 
 def quantize_blockwise(x: torch.Tensor, block: tuple[int, int] = ROW) -> BlockScaled:
@@ -148,27 +162,29 @@ def quantize_blockwise(x: torch.Tensor, block: tuple[int, int] = ROW) -> BlockSc
     of dimensions, or ``(128, 128)`` of a matrix.  Blocks at the end of an axis may be shorter.  fp32, bf16 and fp16 run on
     one kernel launch on CUDA; other floating types are converted to fp32 first.  The result carries no gradient."""
     block = _check_block(block)
+    if x.is_cuda:
+        out = scaled_fused.quantize(x, block is SQUARE or block == SQUARE)
+        if out is not None:
+            return _made(out[0], out[1], block)
     _refuse_vmap("quantize_blockwise", x)
     if not x.is_floating_point() or x.element_size() == 1:
         raise TypeError(f"quantize_blockwise takes fp64, fp32, bf16 or fp16 tensors, got {x.dtype}")
-    if x.dim() == 0:
+    dims = x.dim()
+    if dims == 0:
         raise ValueError("quantize_blockwise needs at least one dimension")
-    x = x.detach()
+    if dims != 2 and block == SQUARE:
+        raise ValueError(f"blocks of (128, 128) need a matrix, got {dims} dimensions")
     if x.dtype == torch.float64:
-        x = x.float()
-    if x.dim() == 2:
-        if x.numel() == 0:
-            return BlockScaled(*_quantize_plain(x, block), block)
-        q = _quantize_2d(x, block)[0]
-        assert q is not None
-        return q
-    shape = _scale_shape(x.shape, block)
+        return quantize_blockwise(x.float(), block)
     if x.numel() == 0:
-        return BlockScaled(x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(shape, dtype=torch.float8_e8m0fnu), block)
-    q = _quantize_2d(x.reshape(-1, x.shape[-1]), block)[0]
-    assert q is not None
-    return BlockScaled(q.codes.unflatten(0, x.shape[:-1]) if x.dim() > 1 else q.codes[0],
-                       q.scales.unflatten(0, x.shape[:-1]) if x.dim() > 1 else q.scales[0], block)
+        shape = _scale_shape(x.shape, block)
+        return _made(x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(shape, dtype=torch.float8_e8m0fnu), block)
+    if x.is_cuda:
+        scaled_fused.declined("quantize", "outside the coverage of the kernel")
+    if dims == 2:
+        return _made(*_quantize_plain(x.detach(), block), block)
+    codes, scales = _quantize_plain(x.detach().reshape(-1, x.shape[-1]), block)
+    return _made(codes.view(x.shape), scales.view(*x.shape[:-1], scales.shape[-1]), block)
 
 
 def _check_bias(bias: torch.Tensor | None, n: int, device: torch.device) -> None:
@@ -188,19 +204,25 @@ def scaled_matmul(a: BlockScaled, b: BlockScaled, bias: torch.Tensor | None = No
     differentiable: :func:`scaled_linear` is the form with gradients."""
     if not isinstance(a, BlockScaled) or not isinstance(b, BlockScaled):
         raise TypeError("scaled_matmul takes BlockScaled operands (see quantize_blockwise)")
+    if a.codes.is_cuda and out_dtype in _HALF:
+        out = scaled_fused.scaled_matmul(a, b, bias, out_dtype)
+        if out is not None:
+            return out
     _refuse_vmap("scaled_matmul", a.codes, a.scales, b.codes, b.scales, bias)
-    if b.codes.dim() != 2:
-        raise ValueError(f"b needs two dimensions, got {b.codes.dim()}")
-    if a.shape[-1] != b.shape[-1]:
-        raise ValueError(f"reduction sizes differ: {a.shape[-1]} vs {b.shape[-1]}")
+    sa, sb = a.codes.shape, b.codes.shape
+    if len(sb) != 2:
+        raise ValueError(f"b needs two dimensions, got {len(sb)}")
+    if sa[-1] != sb[1]:
+        raise ValueError(f"reduction sizes differ: {sa[-1]} vs {sb[1]}")
     if a.codes.device != b.codes.device:
         raise ValueError(f"operands on {a.codes.device} and {b.codes.device}")
-    if out_dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    if out_dtype not in _HALF:
         raise TypeError(f"out_dtype is fp32, bf16 or fp16, got {out_dtype}")
-    n = b.shape[0]
-    _check_bias(bias, n, a.codes.device)
+    n = sb[0]
+    if bias is not None:
+        _check_bias(bias, n, a.codes.device)
     if a.codes.numel() == 0 or n == 0:
-        y = torch.zeros(*a.shape[:-1], n, dtype=torch.float32, device=a.codes.device)
+        y = torch.zeros(*sa[:-1], n, dtype=torch.float32, device=a.codes.device)
         return (y if bias is None else y + bias.detach().float()).to(out_dtype)
     return _product(a, b, None if bias is None else bias.detach(), out_dtype)
 
@@ -240,9 +262,6 @@ class _ScaledLinear(torch.autograd.Function):
         return dx, dw, db, None, None, None
 
 
-_HALF = (torch.float32, torch.bfloat16, torch.float16)
-
-
 def _check_linear(name: str, x: torch.Tensor, weight: "torch.Tensor | BlockScaled", bias: torch.Tensor | None) -> tuple:
     """Checks of the linear entry points; returns ``(K, N, prepared)``."""
     prepared = isinstance(weight, BlockScaled)
@@ -275,27 +294,25 @@ def scaled_linear(x: torch.Tensor, weight: "torch.Tensor | BlockScaled", bias: t
     the fp32 sum.  Sums are fp32; the output has the autocast type or that of ``x``, gradients the types of their tensors.
 
     ``weight`` may be prepared once with ``quantize_blockwise(weight, (128, 128))`` for inference."""
+    prepared = isinstance(weight, BlockScaled)
+    if x.is_cuda:
+        out = scaled_fused.prepared_linear(x, weight, bias) if prepared else scaled_fused.scaled_linear(x, weight, bias)
+        if out is not None:
+            return out
     K, N, prepared = _check_linear("scaled_linear", x, weight, bias)
-    out_dtype = autocast_dtype(x.device.type) or x.dtype
-    if out_dtype not in _HALF:
-        out_dtype = x.dtype
+    out_dtype = _out_dtype(x)
     M = math.prod(x.shape[:-1])
     if M == 0 or N == 0 or K == 0:
         w = weight.dequantize(x.dtype) if prepared else weight.to(x.dtype)
         return torch.nn.functional.linear(x, w, None if bias is None else bias.to(x.dtype)).to(out_dtype)
     if prepared:
-        b = None if bias is None else bias.detach()
-        if x.is_cuda:
-            from ...ops import scaled_fused
-
-            return scaled_fused.prepared_linear(x.detach(), weight, b, out_dtype)
-        return _product(quantize_blockwise(x), weight, b, out_dtype)
+        return _product(quantize_blockwise(x), weight, None if bias is None else bias.detach(), out_dtype)
     need_x, need_w = _grads(x, weight)
-    if x.is_cuda:
-        from ...ops import scaled_fused
-
-        out = scaled_fused.maybe_fused_scaled_linear(x, weight, bias, out_dtype, need_x, need_w)
-        if out is not None:
-            return out
     y = _ScaledLinear.apply(x.reshape(M, K), weight, bias, out_dtype, need_x, need_w)
     return y.view(*x.shape[:-1], N)
+
+
+def _out_dtype(x: torch.Tensor) -> torch.dtype:
+    """The autocast type, or that of ``x``."""
+    dt = autocast_dtype(x.device.type)
+    return dt if dt in _HALF else x.dtype

@@ -21,6 +21,7 @@ from torch.autograd.function import once_differentiable
 
 from ..._core.autocast import autocast_dtype
 from ..._core.collectives import all_reduce_sum
+from ...ops import scaled_fused
 from ..linear._scaled import (
     _HALF,
     ROW,
@@ -28,6 +29,8 @@ from ..linear._scaled import (
     BlockScaled,
     _check_linear,
     _grads,
+    _made,
+    _out_dtype,
     _product,
     _quantize_2d,
     _refuse_vmap,
@@ -44,9 +47,9 @@ def _check(name: str, x: torch.Tensor, weight: torch.Tensor | None, residual: to
         raise ValueError(f"{name}: weight of shape {tuple(weight.shape)} for {x.shape[-1]} features")
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"{name}: residual of shape {tuple(residual.shape)}, input of shape {tuple(x.shape)}")
-    for t in (weight, residual):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{name}: input on {x.device}, weight or residual on {t.device}")
+    dev = x.device
+    if (weight is not None and weight.device != dev) or (residual is not None and residual.device != dev):
+        raise ValueError(f"{name}: input on {dev}, weight or residual on another device")
     if not (math.isfinite(eps) and eps >= 0):
         raise ValueError(f"{name}: eps must be finite and not negative, got {eps}")
 
@@ -93,35 +96,31 @@ def distributed_rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, co
     common type of the two, is the residual of the next block.  Statistics are fp32 or wider; ``y`` is fp32 under autocast
     and has the type of the sum otherwise.  Differentiable in every tensor.  On CUDA with the whole feature axis on one
     rank, fp32, bf16 and fp16 run as one kernel per direction (plus one that adds up the weight's gradient)."""
-    _check("distributed_rms_norm", x, weight, residual, eps)
-    x, residual = _same_type(x, residual)
-    out_dtype = x.dtype if autocast_dtype(x.device.type) is None else torch.promote_types(x.dtype, torch.float32)
     whole = col_group is None or col_group.size() == 1
-    if x.is_cuda and whole and _fusable(x, weight, residual):
-        from ...ops import scaled_fused
-
-        out = scaled_fused.maybe_fused_rms_norm(x, weight, residual, eps, out_dtype, any(_grads(x, weight, residual)))
+    if x.is_cuda and whole:
+        out = scaled_fused.rms_norm(x, weight, residual, eps)
         if out is not None:
             return out[0] if residual is None else out
+    _check("distributed_rms_norm", x, weight, residual, eps)
+    if residual is not None and residual.dtype != x.dtype:
+        x, residual = _same_type(x, residual)
+        return distributed_rms_norm(x, weight, col_group, eps, residual)
+    if x.is_cuda and whole and x.numel() > 0:
+        scaled_fused.declined("rms_norm", "under torch.vmap, in 64 bits, or rows longer than the kernel keeps in registers")
+    out_dtype = x.dtype if autocast_dtype(x.device.type) is None else torch.promote_types(x.dtype, torch.float32)
     y, t, _ = _plain(x, weight, residual, col_group, eps)
     y = y.to(out_dtype)
     return y if residual is None else (y, t)
 
 
-def _fusable(*tensors: torch.Tensor | None) -> bool:
-    """Types that the kernels take, at least one element, no ``torch.vmap`` (the kernels have no batching rules)."""
-    return all(t is None or (t.dtype in _HALF and t.numel() > 0 and not torch._C._functorch.is_batchedtensor(t)) for t in tensors)
-
-
 def _norm_to_codes(x: torch.Tensor, weight: torch.Tensor | None, eps: float, residual: torch.Tensor | None,
                    keep_rstd: bool) -> tuple[BlockScaled, torch.Tensor, torch.Tensor | None]:
     """``(codes, sum, r)``; ``r`` per row."""
-    if x.is_cuda and _fusable(x, weight, residual):
-        from ...ops import scaled_fused
-
-        out = scaled_fused.maybe_fused_rms_quantize(x, weight, eps, residual, keep_rstd)
+    if x.is_cuda:
+        out = scaled_fused.rms_norm_quantize(x, weight, eps, residual, keep_rstd)
         if out is not None:
-            return BlockScaled(out[0], out[1], ROW), (x if out[2] is None else out[2]), out[3]
+            return _made(out[0], out[1], ROW), (x if out[2] is None else out[2]), out[3]
+        scaled_fused.declined("rms_norm_quantize", "in 64 bits, or rows longer than the kernel keeps in registers")
     y, t, r = _plain(x, weight, residual, None, eps)
     return quantize_blockwise(y), t, r.reshape(-1)
 
@@ -131,15 +130,21 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, eps: 
     """Root-mean-square norm with the output in 8 bits (blocks of 128 features, quantised from the unrounded fp32 value):
     a :class:`BlockScaled`, or ``(BlockScaled, x + residual)`` with a residual.  For inference: not differentiable
     (:func:`rms_norm_linear` is), so tensors that want gradients are refused."""
+    if x.is_cuda and not any(_grads(x, weight, residual)):
+        out = scaled_fused.rms_norm_quantize(x, weight, eps, residual, False)
+        if out is not None:
+            q = _made(out[0], out[1], ROW)
+            return q if residual is None else (q, out[2])
     _check("rms_norm_quantize", x, weight, residual, eps)
     _refuse_vmap("rms_norm_quantize", x, weight, residual)
     if any(_grads(x, weight, residual)):
         raise ValueError("rms_norm_quantize has no gradient; use rms_norm_linear, or call it under torch.no_grad()")
-    x, residual = _same_type(x, residual)
-    c = x.shape[-1]
+    if residual is not None and residual.dtype != x.dtype:
+        x, residual = _same_type(x, residual)
+        return rms_norm_quantize(x, weight, eps, residual)
     if x.numel() == 0:
         empty = BlockScaled(x.new_empty(x.shape, dtype=torch.float8_e4m3fn),
-                            x.new_empty((*x.shape[:-1], -(-c // 128)), dtype=torch.float8_e8m0fnu), ROW)
+                            x.new_empty((*x.shape[:-1], -(-x.shape[-1] // 128)), dtype=torch.float8_e8m0fnu), ROW)
         return empty if residual is None else (empty, x + residual)
     q, t, _ = _norm_to_codes(x.detach(), weight, eps, None if residual is None else residual.detach(), False)
     return q if residual is None else (q, t)
@@ -189,6 +194,12 @@ def rms_norm_linear(x: torch.Tensor, norm_weight: torch.Tensor | None, weight: "
     normalised rows are quantised from their unrounded fp32 values and never stored otherwise.  Returns ``y``, or
     ``(y, x + residual)`` with a residual.  Differentiable like :func:`scaled_linear`; a prepared ``weight`` serves
     inference."""
+    prepared = isinstance(weight, BlockScaled)
+    if x.is_cuda:
+        run = scaled_fused.prepared_norm_linear if prepared else scaled_fused.rms_norm_linear
+        out = run(x, norm_weight, weight, bias, residual, eps)
+        if out is not None:
+            return out[0] if residual is None else out
     K, N, prepared = _check_linear("rms_norm_linear", x, weight, bias)
     _check("rms_norm_linear", x, norm_weight, residual, eps)
     _refuse_vmap("rms_norm_linear", norm_weight, residual)
@@ -196,10 +207,10 @@ def rms_norm_linear(x: torch.Tensor, norm_weight: torch.Tensor | None, weight: "
         raise TypeError("rms_norm_linear takes fp32, bf16 or fp16 tensors")
     if prepared and any(_grads(norm_weight, residual)):
         raise ValueError("rms_norm_linear: a prepared weight (BlockScaled) serves inference only; call it under torch.no_grad()")
-    out_dtype = autocast_dtype(x.device.type) or x.dtype
-    x, residual = _same_type(x, residual)
-    if out_dtype not in _HALF:
-        out_dtype = x.dtype
+    if residual is not None and residual.dtype != x.dtype:
+        x, residual = _same_type(x, residual)
+        return rms_norm_linear(x, norm_weight, weight, bias, eps, residual)
+    out_dtype = _out_dtype(x)
     M = math.prod(x.shape[:-1])
     if M == 0 or N == 0 or K == 0:
         h, t, _ = _plain(x, norm_weight, residual, None, eps)
@@ -207,23 +218,10 @@ def rms_norm_linear(x: torch.Tensor, norm_weight: torch.Tensor | None, weight: "
         y = torch.nn.functional.linear(h.float(), w, None if bias is None else bias.float()).to(out_dtype)
         return y if residual is None else (y, t)
     if prepared:
-        x, b, r = x.detach(), None if bias is None else bias.detach(), None if residual is None else residual.detach()
-        out = None
-        if x.is_cuda:
-            from ...ops import scaled_fused
-
-            out = scaled_fused.maybe_prepared_norm_linear(x, norm_weight, weight, b, r, eps, out_dtype)
-        if out is None:
-            q, t, _ = _norm_to_codes(x, norm_weight, eps, r, False)
-            out = _product(q, weight, b, out_dtype), t
-        return out[0] if residual is None else out
+        q, t, _ = _norm_to_codes(x.detach(), norm_weight, eps, None if residual is None else residual.detach(), False)
+        y = _product(q, weight, None if bias is None else bias.detach(), out_dtype)
+        return y if residual is None else (y, t)
     gx, gn, gw, gr = _grads(x, norm_weight, weight, residual)
-    if x.is_cuda:
-        from ...ops import scaled_fused
-
-        out = scaled_fused.maybe_fused_rms_norm_linear(x, norm_weight, weight, bias, residual, eps, out_dtype, gx or gn or gr, gw)
-        if out is not None:
-            return out[0] if residual is None else out
     out = _RmsNormLinear.apply(x.reshape(M, K), norm_weight, weight, bias, eps, None if residual is None else residual.reshape(M, K),
                                out_dtype, gx or gn or gr, gw)
     if residual is None:

@@ -6,6 +6,7 @@
 // The kernel library is loaded by Python, which hands its entry points over in init(): the binding links against torch
 // only.
 #include <ATen/ATen.h>
+#include <ATen/autocast_mode.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -13,7 +14,9 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <array>
 #include <atomic>
+#include <cmath>
 #include <optional>
 
 #include "scaled_abi.h"
@@ -29,6 +32,7 @@ struct Api {
   decltype(&jb_scaled_gemm) gemm = nullptr;
   decltype(&jb_quantize) quantize = nullptr;
   decltype(&jb_column_sum) column_sum = nullptr;
+  decltype(&jb_rms_max_cols) rms_max_cols = nullptr;
   decltype(&jb_rms_norm_fwd) rms_fwd = nullptr;
   decltype(&jb_rms_bwd_parts) rms_bwd_parts = nullptr;
   decltype(&jb_rms_norm_bwd) rms_bwd = nullptr;
@@ -506,14 +510,73 @@ struct RmsNormLinear : public Function<RmsNormLinear> {
 };
 
 // ------------------------------------------------------------------------------------------------ Python
+// Every entry point answers None to a call that is not an ordinary one for the kernels: other types, devices or shapes that
+// do not fit, empty tensors, tensors wrapped by a transform.  The caller then takes its general path, which raises the
+// error or computes the call in torch operations.
 py::object give(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
 
-py::tuple py_quantize(const Tensor& x, bool square, bool rows, bool cols, const Optional& rstd,
-                      const Optional& gain, int sum_type) {
+bool wrapped(const Tensor& t) {
+  const c10::DispatchKeySet k = t.unsafeGetTensorImpl()->key_set();
+  return k.has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Python}));
+}
+bool float_type(const Tensor& t) {
+  const at::ScalarType s = t.scalar_type();
+  return s == at::kFloat || s == at::kBFloat16 || s == at::kHalf;
+}
+bool ordinary(const Tensor& t, const Tensor& like) {
+  return t.layout() == at::kStrided && t.device() == like.device() && t.is_cuda() && !wrapped(t) && t.numel() > 0;
+}
+bool vector_of(const Optional& t, int64_t n, const Tensor& like) {
+  return !t.has_value() || (float_type(*t) && ordinary(*t, like) && t->dim() == 1 && t->size(0) == n);
+}
+bool matrix_codes(const Tensor& codes, const Tensor& scales, bool square, const Tensor& like) {
+  if (codes.scalar_type() != CODES || scales.scalar_type() != SCALES || !ordinary(codes, like) || !ordinary(scales, like)) return false;
+  const int64_t nb = (codes.size(-1) + 127) / 128;
+  if (square) return codes.dim() == 2 && scales.dim() == 2 && scales.size(0) == (codes.size(0) + 127) / 128 && scales.size(1) == nb;
+  return codes.dim() >= 1 && scales.dim() == codes.dim() && scales.size(-1) == nb && scales.numel() / nb == codes.numel() / codes.size(-1);
+}
+bool norm_args(const Tensor& x, const Optional& gain, const Optional& residual, double eps) {
+  if (!float_type(x) || x.dim() < 1 || !ordinary(x, x) || x.size(-1) > api.rms_max_cols() || !(eps >= 0.0) || std::isinf(eps)) return false;
+  if (!vector_of(gain, x.size(-1), x)) return false;
+  return !residual.has_value() || (residual->scalar_type() == x.scalar_type() && ordinary(*residual, x) && residual->sizes() == x.sizes());
+}
+bool wants(const Tensor& t) { return t.requires_grad(); }
+bool wants(const Optional& t) { return t.has_value() && t->requires_grad(); }
+
+// Type of a layer's output: that of autocast where it is on.
+int autocast_type(const Tensor& x) {
+  if (!at::autocast::is_autocast_enabled(at::kCUDA)) return type_of(x.scalar_type());
+  const at::ScalarType t = at::autocast::get_autocast_dtype(at::kCUDA);
+  return t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : type_of(x.scalar_type());
+}
+
+std::array<Tensor, 64> status_words;                 // per device, set by Python when it first meets one
+void set_status(int64_t device, const Tensor& word) { status_words.at(device) = word; }
+const Tensor& status_of(const Tensor& t) {
+  const Tensor& w = status_words.at(t.device().index());
+  TORCH_CHECK(w.defined(), "no status word for device ", t.device().index());
+  return w;
+}
+
+py::object py_quantize(const Tensor& x, bool square, bool rows, bool cols, const Optional& rstd, const Optional& gain, int sum_type) {
+  if (!float_type(x) || x.dim() < 1 || !ordinary(x, x) || (square && x.dim() != 2) || (cols && x.dim() != 2)) return py::none();
+  if (rstd.has_value() && (x.dim() != 2 || rstd->scalar_type() != at::kFloat || !rstd->is_contiguous() || !vector_of(rstd, x.size(0), x))) return py::none();
+  if (!vector_of(gain, x.size(-1), x)) return py::none();
   const Quantized q = quantize(x, square, rows, cols, opt(rstd), opt(gain), sum_type);
   return py::make_tuple(q.rows ? give(q.rows->code_view()) : py::none(), q.rows ? give(q.rows->scale_view()) : py::none(),
                         q.cols ? give(q.cols->code_view()) : py::none(), q.cols ? give(q.cols->scale_view()) : py::none(),
                         give(q.sums));
+}
+
+py::object py_quantize_any(const Tensor& x, bool square) {
+  if (!float_type(x) || x.dim() < 1 || !ordinary(x, x) || (square && x.dim() != 2)) return py::none();
+  const Quantized q = quantize(x, square, true, false, Tensor(), Tensor(), -1);
+  Tensor codes = q.rows->code_view(), scales = q.rows->scale_view();
+  if (x.dim() != 2) {              // splitting the rows of a strided matrix is a view
+    codes = codes.view(x.sizes());
+    scales = scales.view(with_last(x, scales.size(1)));
+  }
+  return py::make_tuple(give(codes), give(scales));
 }
 
 // A public operand: codes that TMA cannot address (rows not on 16-byte boundaries, or not contiguous) are copied once.
@@ -544,18 +607,21 @@ JbScaledOperand describe(const Codes& c) {
   return o;
 }
 
-Tensor py_scaled_matmul(const Tensor& a_codes, const Tensor& a_scales, bool a_square, const Tensor& b_codes, const Tensor& b_scales,
-                        bool b_square, const Optional& bias, int out_type, const Tensor& status) {
+py::object py_scaled_matmul(const Tensor& a_codes, const Tensor& a_scales, bool a_square, const Tensor& b_codes, const Tensor& b_scales,
+                            bool b_square, const Optional& bias, int out_type) {
+  if (!matrix_codes(a_codes, a_scales, a_square, a_codes) || !matrix_codes(b_codes, b_scales, b_square, a_codes) || b_codes.dim() != 2 ||
+      a_codes.size(-1) != b_codes.size(1) || !vector_of(bias, b_codes.size(0), a_codes))
+    return py::none();
   const c10::cuda::CUDAGuard guard(a_codes.device());
   const Codes a = operand_of(a_codes, a_scales, a_square), b = operand_of(b_codes, b_scales, b_square);
-  return product(describe(a), describe(b), a.cols, opt(bias), out_type, with_last(a_codes, b.rows), a_codes, status);
+  return give(product(describe(a), describe(b), a.cols, opt(bias), out_type, with_last(a_codes, b.rows), a_codes, status_of(a_codes)));
 }
 
-py::tuple py_rms_quantize(const Tensor& x, const Optional& gain, double eps, const Optional& residual,
-                          bool want_rstd) {
+py::object py_rms_quantize(const Tensor& x, const Optional& gain, double eps, const Optional& residual, bool want_rstd) {
+  if (!norm_args(x, gain, residual, eps)) return py::none();
   const Normed n = rms_forward(x, opt(gain), eps, opt(residual), -1, true, want_rstd);
   Tensor codes = n.codes->code_view(), scales = n.codes->scale_view();
-  if (x.dim() != 2) {              // splitting the rows of a strided matrix is a view
+  if (x.dim() != 2) {
     codes = codes.view(x.sizes());
     scales = scales.view(with_last(x, scales.size(1)));
   }
@@ -563,36 +629,49 @@ py::tuple py_rms_quantize(const Tensor& x, const Optional& gain, double eps, con
 }
 
 // Inference forms with a prepared weight: quantisation (with or without the norm) and product, two launches.
-Tensor py_linear_prepared(const Tensor& x, const Tensor& w_codes, const Tensor& w_scales, bool w_square,
-                          const Optional& bias, int out_type, const Tensor& status) {
+py::object py_linear_prepared(const Tensor& x, const Tensor& w_codes, const Tensor& w_scales, bool w_square, const Optional& bias) {
+  if (!float_type(x) || x.dim() < 1 || !ordinary(x, x) || !matrix_codes(w_codes, w_scales, w_square, x) || w_codes.dim() != 2 ||
+      w_codes.size(1) != x.size(-1) || !vector_of(bias, w_codes.size(0), x) || (at::GradMode::is_enabled() && (wants(x) || wants(bias))))
+    return py::none();
   const c10::cuda::CUDAGuard guard(x.device());
   const Quantized q = quantize(x, false, true, false, Tensor(), Tensor(), -1);
   const Codes w = operand_of(w_codes, w_scales, w_square);
-  return product(q.rows->operand(), describe(w), w.cols, opt(bias), out_type, with_last(x, w.rows), x, status);
+  return give(product(q.rows->operand(), describe(w), w.cols, opt(bias), autocast_type(x), with_last(x, w.rows), x, status_of(x)));
 }
-py::tuple py_norm_linear_prepared(const Tensor& x, const Optional& gain, double eps, const Optional& residual,
-                                  const Tensor& w_codes, const Tensor& w_scales, bool w_square, const Optional& bias,
-                                  int out_type, const Tensor& status) {
+py::object py_norm_linear_prepared(const Tensor& x, const Optional& gain, double eps, const Optional& residual, const Tensor& w_codes,
+                                   const Tensor& w_scales, bool w_square, const Optional& bias) {
+  if (!norm_args(x, gain, residual, eps) || !matrix_codes(w_codes, w_scales, w_square, x) || w_codes.dim() != 2 ||
+      w_codes.size(1) != x.size(-1) || !vector_of(bias, w_codes.size(0), x) ||
+      (at::GradMode::is_enabled() && (wants(x) || wants(gain) || wants(residual) || wants(bias))))
+    return py::none();
   const c10::cuda::CUDAGuard guard(x.device());
   const Normed n = rms_forward(x, opt(gain), eps, opt(residual), -1, true, false);
   const Codes w = operand_of(w_codes, w_scales, w_square);
-  return py::make_tuple(give(product(n.codes->operand(), describe(w), w.cols, opt(bias), out_type, with_last(x, w.rows), x, status)),
+  return py::make_tuple(give(product(n.codes->operand(), describe(w), w.cols, opt(bias), autocast_type(x), with_last(x, w.rows), x, status_of(x))),
                         give(n.sum));
 }
 
-Tensor py_scaled_linear(const Tensor& x, const Tensor& w, const Optional& b, int out_type, bool need_x, bool need_w,
-                        const Tensor& status) {
-  return ScaledLinear::apply(x, w, b, static_cast<int64_t>(out_type), need_x, need_w, status);
+bool weight_args(const Tensor& x, const Tensor& w, const Optional& b) {
+  return float_type(w) && ordinary(w, x) && w.dim() == 2 && w.size(1) == x.size(-1) && vector_of(b, w.size(0), x);
+}
+py::object py_scaled_linear(const Tensor& x, const Tensor& w, const Optional& b) {
+  if (!float_type(x) || x.dim() < 1 || !ordinary(x, x) || !weight_args(x, w, b)) return py::none();
+  const bool grad = at::GradMode::is_enabled();
+  return give(ScaledLinear::apply(x, w, b, static_cast<int64_t>(autocast_type(x)), grad && wants(x), grad && wants(w), status_of(x)));
 }
 py::tuple pair_of(const variable_list& v) { return py::make_tuple(give(v[0]), v.size() > 1 ? give(v[1]) : py::none()); }
-py::tuple py_rms_norm(const Tensor& x, const Optional& gain, const Optional& residual, double eps,
-                      int y_type, bool need) {
-  return pair_of(RmsNorm::apply(x, gain, residual, eps, static_cast<int64_t>(y_type), need));
+py::object py_rms_norm(const Tensor& x, const Optional& gain, const Optional& residual, double eps) {
+  if (!norm_args(x, gain, residual, eps)) return py::none();
+  const bool need = at::GradMode::is_enabled() && (wants(x) || wants(gain) || wants(residual));
+  const int64_t y_type = at::autocast::is_autocast_enabled(at::kCUDA) ? 0 : type_of(x.scalar_type());
+  return pair_of(RmsNorm::apply(x, gain, residual, eps, y_type, need));
 }
-py::tuple py_rms_norm_linear(const Tensor& x, const Optional& gain, const Tensor& w, const Optional& b,
-                             const Optional& residual, double eps, int out_type, bool need_h, bool need_w,
-                             const Tensor& status) {
-  return pair_of(RmsNormLinear::apply(x, gain, w, b, residual, eps, static_cast<int64_t>(out_type), need_h, need_w, status));
+py::object py_rms_norm_linear(const Tensor& x, const Optional& gain, const Tensor& w, const Optional& b, const Optional& residual,
+                              double eps) {
+  if (!norm_args(x, gain, residual, eps) || !weight_args(x, w, b)) return py::none();
+  const bool grad = at::GradMode::is_enabled();
+  return pair_of(RmsNormLinear::apply(x, gain, w, b, residual, eps, static_cast<int64_t>(autocast_type(x)),
+                                      grad && (wants(x) || wants(gain) || wants(residual)), grad && wants(w), status_of(x)));
 }
 
 void init(const py::dict& entry) {
@@ -602,6 +681,7 @@ void init(const py::dict& entry) {
   take(api.gemm, "jb_scaled_gemm");
   take(api.quantize, "jb_quantize");
   take(api.column_sum, "jb_column_sum");
+  take(api.rms_max_cols, "jb_rms_max_cols");
   take(api.rms_fwd, "jb_rms_norm_fwd");
   take(api.rms_bwd_parts, "jb_rms_bwd_parts");
   take(api.rms_bwd, "jb_rms_norm_bwd");
@@ -611,6 +691,8 @@ void init(const py::dict& entry) {
 
 PYBIND11_MODULE(_jb_torch, m) {
   m.def("init", &init);
+  m.def("set_status", &set_status);
+  m.def("quantize_any", &py_quantize_any);
   m.def("launches", [] { return launches.load(std::memory_order_relaxed); });
   m.def("quantize", &py_quantize);
   m.def("scaled_matmul", &py_scaled_matmul);
