@@ -66,10 +66,10 @@ struct JbRmsBwd {
 extern "C" {
 int jb_scaled_gemm(const JbScaledOperand* a, const JbScaledOperand* b, long long K, void* out, long long ldo, int out_type,
                    const void* bias, int bias_type, int sm_count, int* status, void* stream);
-int jb_quantize(const JbQuant* q, void* stream);
+int jb_quantize(const JbQuant* q, int sm_count, void* stream);
 int jb_column_sum(const float* part, int P, int C, void* out, int out_type, void* stream);
 int jb_rms_max_cols();
 int jb_rms_norm_fwd(const JbRms* q, int sm_count, void* stream);
-int jb_rms_bwd_parts(int rows, int cols, int sm_count);
-int jb_rms_norm_bwd(const JbRmsBwd* q, int sm_count, void* stream);
+int jb_rms_bwd_parts(const JbRmsBwd* q, int sm_count);
+int jb_rms_norm_bwd(const JbRmsBwd* q, int sm_count, int* status, void* stream);
 }

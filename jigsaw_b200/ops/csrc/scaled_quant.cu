@@ -48,11 +48,16 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], float inv) {
   return make_uint2(codes4(code_input<CHECKED>(v[0], inv), code_input<CHECKED>(v[1], inv), code_input<CHECKED>(v[2], inv), code_input<CHECKED>(v[3], inv)),
                     codes4(code_input<CHECKED>(v[4], inv), code_input<CHECKED>(v[5], inv), code_input<CHECKED>(v[6], inv), code_input<CHECKED>(v[7], inv)));
 }
+// max(m, |a|, |b|), NaN if one of them is.
+__device__ __forceinline__ float max_abs3(float m, float a, float b) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(a), "f"(b));
+  return r;
+}
+
 // Scale byte and codes of a block of 128 values held by 16 neighbouring lanes, eight each.
 __device__ __forceinline__ uint32_t block_of_16_lanes(const float (&v)[8], uint2& codes) {
-  uint32_t m = 0u;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) m = max(m, magnitude(v[e]));
+  uint32_t m = magnitude(max_abs3(max_abs3(max_abs3(max_abs3(0.f, v[0], v[1]), v[2], v[3]), v[4], v[5]), v[6], v[7]));
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (__any_sync(0xffffffffu, m >= INF_BITS)) {
@@ -190,168 +195,243 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
 }
 
 // ---------------------------------------------------------------- tiles of 128 x 128
-// max(m, |a|, |b|), NaN if one of them is.
-__device__ __forceinline__ float max_abs3(float m, float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
-  return r;
+// 16 bytes from global to shared memory behind the thread's back; `bytes` < 16 leaves zeros in the rest.
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
 struct TileShared {
-  __align__(16) uint8_t turned[128 * 128];
-  __align__(16) uint32_t col_mag[16][128];
-  __align__(16) float col_sum[16][128];
-  __align__(16) float col_inv[128];
+  union {                                // the magnitudes and sums are read before the codes turn
+    uint8_t turned[128 * 128];
+    struct {
+      uint32_t col_mag[16][128];
+      float col_sum[16][128];
+    };
+  };
+  float col_inv[128];
   uint32_t row_mag[16];
 };
+constexpr int QT_SHARED = (sizeof(TileShared) + 127) / 128 * 128;
+// How a tile is read: element by element, with wide loads, or by copies into shared memory one tile ahead.
+enum : int { QT_PLAIN = 0, QT_WIDE = 1, QT_AHEAD = 2 };
+template <typename T, int MODE>
+constexpr int quant_tile_smem() { return QT_SHARED + (MODE == QT_AHEAD ? 2 * 128 * 128 * static_cast<int>(sizeof(T)) : 0); }
 
-// One CTA, one tile, 32 values a thread (warp w: rows 8 w .. 8 w + 7, lane l: columns 4 l .. 4 l + 3), so that two CTAs of
-// sixteen warps share an SM.  Scales by row come from warp reductions, by column through shared memory, or from the
-// whole tile; the transposed codes turn in shared memory, eight bytes of a column at a time.
-template <typename T, bool VEC, bool NORM>
-__global__ void __launch_bounds__(512, 2) quant_tile_kernel(const QuantArgs a) {
-  __shared__ TileShared sh;
+// Tiles of 128 x 128, 32 values a thread (warp w: rows 8 w .. 8 w + 7, lane l: columns 4 l .. 4 l + 3).  Scales by row come
+// from warp reductions, by column through shared memory, or from the whole tile; the transposed codes turn in shared
+// memory, eight bytes of a column at a time.  A CTA takes tiles in steps of the grid; of 16-bit values it has the next tile
+// copied into shared memory while it works on the present one (8192 x 11008 bf16, both layouts: 134 us with loads, which
+// the warps waited for half of the time).  Two fp32 tiles ahead would leave room for one CTA an SM, which is slower than
+// loads (11001 x 4100: 48 us against 39).
+template <typename T, int MODE, bool NORM>
+__global__ void __launch_bounds__(512, 2) quant_tile_kernel(const QuantArgs a, int tiles_r, int tiles) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  TileShared& sh = *reinterpret_cast<TileShared*>(smem);
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int tile_r = blockIdx.x, tile_c = blockIdx.y;
-  const long long row0 = static_cast<long long>(tile_r) * 128 + warp * 8;
-  const int col = tile_c * 128 + lane * 4;
-  const int live = min(4, max(0, a.cols - col));
-  const int live_rows = static_cast<int>(max(0LL, min(8LL, a.rows - row0)));
-  float v[8][4];
-  {
-    const T* x = static_cast<const T*>(a.x) + row0 * a.ldx + col;
+  constexpr int E16 = 16 / static_cast<int>(sizeof(T));          // elements of a 16-byte copy
+  constexpr int TILE_BYTES = 128 * 128 * static_cast<int>(sizeof(T));
+  // Thread q of the copy takes 16 bytes at column (q % PER_ROW) E16 of every (512 / PER_ROW)-th row.
+  constexpr int PER_ROW = 128 / E16, ROW_STEP = 512 / PER_ROW;
+  const int copy_r = threadIdx.x / PER_ROW, copy_c = threadIdx.x % PER_ROW * E16;
+  const long long copy_step = a.ldx * ROW_STEP;
+  auto prefetch = [&](int tr, int tc, int stage) {
+    const int r = tr * 128 + copy_r, c = tc * 128 + copy_c;
+    const T* src = static_cast<const T*>(a.x) + r * a.ldx + c;
+    const uint32_t dst = smem_u32(smem) + QT_SHARED + stage * TILE_BYTES + threadIdx.x * 16;
+    const int rows = c < a.cols ? a.rows - r : 0;                // cols is a multiple of E16
 #pragma unroll
-    for (int i = 0; i < 8; ++i) load_vec<T, 4, VEC>(x + i * a.ldx, i < live_rows ? live : 0, v[i]);
-  }
-  if constexpr (NORM) {
-    float g[4] = {1.f, 1.f, 1.f, 1.f};
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < live) g[j] = gain_at(a.gain, a.gain_type, col + j);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float r = i < live_rows ? __ldg(a.rstd + row0 + i) : 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[i][j] = v[i][j] * r * g[j];
+    for (int k = 0; k < 128 / ROW_STEP; ++k) {
+      const bool in = k * ROW_STEP < rows;
+      copy16_async(dst + k * 512 * 16, in ? src : static_cast<const T*>(a.x), in ? 16 : 0);
+      src += copy_step;
     }
-  }
-  uint32_t cm[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float m = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) m = max_abs3(m, v[i][j], v[i + 1][j]);
-    cm[j] = magnitude(m);
-  }
-  if (a.colsum != nullptr) {
-    float t[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      t[j] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t[j] += v[i][j];
-    }
-    *reinterpret_cast<float4*>(&sh.col_sum[warp][lane * 4]) = make_float4(t[0], t[1], t[2], t[3]);
-  }
-  const uint32_t top = max(max(cm[0], cm[1]), max(cm[2], cm[3]));
-  auto share = [&](uint32_t most) {
-    if (a.square) {
-      const uint32_t m = __reduce_max_sync(0xffffffffu, most);
-      if (lane == 0) sh.row_mag[warp] = m;
-    } else if (a.codes_t != nullptr) {
-      *reinterpret_cast<uint4*>(&sh.col_mag[warp][lane * 4]) = make_uint4(cm[0], cm[1], cm[2], cm[3]);
+    copies_commit();
+  };
+  // tiles run down the rows first; the grid's step in both directions, so that no tile costs a division
+  int tile_r = blockIdx.x % tiles_r, tile_c = blockIdx.x / tiles_r;
+  const int step_r = gridDim.x % tiles_r, step_c = gridDim.x / tiles_r;
+  auto advance = [&](int& r, int& c) {
+    r += step_r;
+    c += step_c;
+    if (r >= tiles_r) {
+      r -= tiles_r;
+      ++c;
     }
   };
-  share(top);
-  // not a number among the values: the rest of the tile runs on finite magnitudes, and such values leave as NaN codes
-  const bool checked = __syncthreads_or(top >= INF_BITS) != 0;
-  if (checked) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      cm[j] = 0u;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) cm[j] = max(cm[j], finite_magnitude(v[i][j]));
-    }
-    share(max(max(cm[0], cm[1]), max(cm[2], cm[3])));
-    __syncthreads();
-  }
-  uint32_t square_byte = 0u;
-  if (a.square) {
-    uint32_t m = 0u;
-#pragma unroll
-    for (int w = 0; w < 16; ++w) m = max(m, sh.row_mag[w]);
-    square_byte = scale_byte(m);
-    if (threadIdx.x == 0) a.scales[tile_r * a.scale_row + tile_c * a.scale_k] = static_cast<uint8_t>(square_byte);
-  } else if (a.codes_t != nullptr && threadIdx.x < 128) {
-    uint32_t m = 0u;
-#pragma unroll
-    for (int w = 0; w < 16; ++w) m = max(m, sh.col_mag[w][threadIdx.x]);
-    const uint32_t byte = scale_byte(m);
-    sh.col_inv[threadIdx.x] = inverse_scale(byte);
-    const int c = tile_c * 128 + threadIdx.x;
-    if (c < a.cols) a.scales_t[c * a.scale_t_row + tile_r * a.scale_t_k] = static_cast<uint8_t>(byte);
-  }
-  if (a.colsum != nullptr && threadIdx.x >= 128 && threadIdx.x < 256 && tile_c * 128 + threadIdx.x - 128 < a.cols) {
-    float t = 0.f;
-#pragma unroll
-    for (int w = 0; w < 16; ++w) t += sh.col_sum[w][threadIdx.x - 128];
-    a.colsum[static_cast<long long>(tile_r) * a.cols + tile_c * 128 + threadIdx.x - 128] = t;
-  }
-  if (checked) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[i][j] = code_input<true>(v[i][j], 1.f);      // NaN for every value that is not finite
-  }
-  if (a.codes != nullptr) {
-    uint32_t mine = 0u;
-    uint8_t* out = a.codes + row0 * a.pitch + col;
-    const bool in_pitch = col < a.pitch;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t byte = square_byte;
-      if (!a.square) {
-        uint32_t m = magnitude(max_abs3(max_abs3(0.f, v[i][0], v[i][1]), v[i][2], v[i][3]));
-        if (checked)
-          m = max(max(finite_magnitude(v[i][0]), finite_magnitude(v[i][1])), max(finite_magnitude(v[i][2]), finite_magnitude(v[i][3])));
-        byte = scale_byte(__reduce_max_sync(0xffffffffu, m));
-        if (lane == i) mine = byte;
+  int stage = 0;
+  if constexpr (MODE == QT_AHEAD) prefetch(tile_r, tile_c, 0);
+  for (int t = blockIdx.x; t < tiles; t += gridDim.x, stage ^= 1, advance(tile_r, tile_c)) {
+    const long long row0 = static_cast<long long>(tile_r) * 128 + warp * 8;
+    const int col = tile_c * 128 + lane * 4;
+    const int live = min(4, max(0, a.cols - col));
+    const int live_rows = static_cast<int>(max(0LL, min(8LL, a.rows - row0)));
+    float v[8][4];
+    if constexpr (MODE == QT_AHEAD) {
+      if (t + gridDim.x < tiles) {
+        int next_r = tile_r, next_c = tile_c;
+        advance(next_r, next_c);
+        prefetch(next_r, next_c, stage ^ 1);
+        copies_wait<1>();
+      } else {
+        copies_wait<0>();
       }
-      const float inv = inverse_scale(byte);
-      if (i < live_rows && in_pitch)
-        *reinterpret_cast<uint32_t*>(out) = codes4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-      out += a.pitch;
-    }
-    if (!a.square && lane < live_rows) a.scales[(row0 + lane) * a.scale_row + tile_c * a.scale_k] = static_cast<uint8_t>(mine);
-  }
-  if (a.codes_t != nullptr) {
-    float inv[4];
-    if (a.square) {
-      inv[0] = inv[1] = inv[2] = inv[3] = inverse_scale(square_byte);
+      __syncthreads();               // this tile is there, and the last one's turned codes have been read
+      const T* in = reinterpret_cast<const T*>(smem + QT_SHARED + stage * TILE_BYTES) + (warp * 8) * 128 + lane * 4;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        __align__(16) T e[4];
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(in + i * 128);
+        else *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(in + i * 128);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][j] = to_f32<T>(e[j]);
+      }
     } else {
       __syncthreads();
-      const float4 f = *reinterpret_cast<const float4*>(&sh.col_inv[lane * 4]);
-      inv[0] = f.x; inv[1] = f.y; inv[2] = f.z; inv[3] = f.w;
+      const T* x = static_cast<const T*>(a.x) + row0 * a.ldx + col;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) load_vec<T, 4, MODE == QT_WIDE>(x + i * a.ldx, i < live_rows ? live : 0, v[i]);
     }
+    if constexpr (NORM) {
+      float g[4] = {1.f, 1.f, 1.f, 1.f};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < live) g[j] = gain_at(a.gain, a.gain_type, col + j);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float r = i < live_rows ? __ldg(a.rstd + row0 + i) : 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][j] = v[i][j] * r * g[j];
+      }
+    }
+    uint32_t cm[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      uint2 q;
-      q.x = codes4(v[0][j] * inv[j], v[1][j] * inv[j], v[2][j] * inv[j], v[3][j] * inv[j]);
-      q.y = codes4(v[4][j] * inv[j], v[5][j] * inv[j], v[6][j] * inv[j], v[7][j] * inv[j]);
-      // piece `warp` of column 4 lane + j, at a place that differs between the sixteen lanes of a store's half warp
-      *reinterpret_cast<uint2*>(sh.turned + (lane * 4 + j) * 128 + ((warp ^ (lane & 15)) << 3)) = q;
-    }
-    __syncthreads();
+      float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int c = warp * 8 + i * 4 + (lane >> 3);
-      const int piece = lane & 7, turn = (c >> 2) & 15;
-      uint4 q = *reinterpret_cast<const uint4*>(sh.turned + c * 128 + ((((2 * piece) ^ turn) & ~1) << 3));
-      if (turn & 1) q = make_uint4(q.z, q.w, q.x, q.y);
-      const long long at = static_cast<long long>(tile_r) * 128 + piece * 16;
-      if (tile_c * 128 + c < a.cols && at < a.pitch_t)
-        *reinterpret_cast<uint4*>(a.codes_t + (static_cast<long long>(tile_c) * 128 + c) * a.pitch_t + at) = q;
+      for (int i = 0; i < 8; i += 2) m = max_abs3(m, v[i][j], v[i + 1][j]);
+      cm[j] = magnitude(m);
+    }
+    if (a.colsum != nullptr) {
+      float s[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[j] += v[i][j];
+      }
+      *reinterpret_cast<float4*>(&sh.col_sum[warp][lane * 4]) = make_float4(s[0], s[1], s[2], s[3]);
+    }
+    const uint32_t top = max(max(cm[0], cm[1]), max(cm[2], cm[3]));
+    auto share = [&](uint32_t most) {
+      if (a.square) {
+        const uint32_t m = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) sh.row_mag[warp] = m;
+      } else if (a.codes_t != nullptr) {
+        *reinterpret_cast<uint4*>(&sh.col_mag[warp][lane * 4]) = make_uint4(cm[0], cm[1], cm[2], cm[3]);
+      }
+    };
+    share(top);
+    // not a number among the values: the rest of the tile runs on finite magnitudes, and such values leave as NaN codes
+    const bool checked = __syncthreads_or(top >= INF_BITS) != 0;
+    if (checked) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        cm[j] = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) cm[j] = max(cm[j], finite_magnitude(v[i][j]));
+      }
+      share(max(max(cm[0], cm[1]), max(cm[2], cm[3])));
+      __syncthreads();
+    }
+    uint32_t square_byte = 0u;
+    if (a.square) {
+      uint32_t m = 0u;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) m = max(m, sh.row_mag[w]);
+      square_byte = scale_byte(m);
+      if (threadIdx.x == 0) a.scales[tile_r * a.scale_row + tile_c * a.scale_k] = static_cast<uint8_t>(square_byte);
+    } else if (a.codes_t != nullptr && threadIdx.x < 128) {
+      uint32_t m = 0u;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) m = max(m, sh.col_mag[w][threadIdx.x]);
+      const uint32_t byte = scale_byte(m);
+      sh.col_inv[threadIdx.x] = inverse_scale(byte);
+      const int c = tile_c * 128 + threadIdx.x;
+      if (c < a.cols) a.scales_t[c * a.scale_t_row + tile_r * a.scale_t_k] = static_cast<uint8_t>(byte);
+    }
+    if (a.colsum != nullptr && threadIdx.x >= 128 && threadIdx.x < 256 && tile_c * 128 + threadIdx.x - 128 < a.cols) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) s += sh.col_sum[w][threadIdx.x - 128];
+      a.colsum[static_cast<long long>(tile_r) * a.cols + tile_c * 128 + threadIdx.x - 128] = s;
+    }
+    if (checked) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][j] = code_input<true>(v[i][j], 1.f);      // NaN for every value that is not finite
+    }
+    if (a.codes != nullptr) {
+      // lane i holds the scale of row i: one computation for eight rows
+      uint32_t byte = square_byte;
+      if (!a.square) {
+        uint32_t mine = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t m = magnitude(max_abs3(max_abs3(0.f, v[i][0], v[i][1]), v[i][2], v[i][3]));
+          if (checked)
+            m = max(max(finite_magnitude(v[i][0]), finite_magnitude(v[i][1])), max(finite_magnitude(v[i][2]), finite_magnitude(v[i][3])));
+          m = __reduce_max_sync(0xffffffffu, m);
+          if (lane == i) mine = m;
+        }
+        byte = scale_byte(mine);
+        if (lane < live_rows) a.scales[(row0 + lane) * a.scale_row + tile_c * a.scale_k] = static_cast<uint8_t>(byte);
+      }
+      const float row_inv = inverse_scale(byte);
+      uint8_t* out = a.codes + row0 * a.pitch + col;
+      const bool in_pitch = col < a.pitch;
+      {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float inv = __shfl_sync(0xffffffffu, row_inv, i);
+          if (in_pitch && i < live_rows) *reinterpret_cast<uint32_t*>(out) = codes4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+          out += a.pitch;
+        }
+      }
+    }
+    if (a.codes_t != nullptr) {
+      float inv[4];
+      if (a.square) {
+        inv[0] = inv[1] = inv[2] = inv[3] = inverse_scale(square_byte);
+        if (a.colsum != nullptr) __syncthreads();        // the sums have been read
+      } else {
+        __syncthreads();
+        const float4 f = *reinterpret_cast<const float4*>(&sh.col_inv[lane * 4]);
+        inv[0] = f.x; inv[1] = f.y; inv[2] = f.z; inv[3] = f.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint2 q;
+        q.x = codes4(v[0][j] * inv[j], v[1][j] * inv[j], v[2][j] * inv[j], v[3][j] * inv[j]);
+        q.y = codes4(v[4][j] * inv[j], v[5][j] * inv[j], v[6][j] * inv[j], v[7][j] * inv[j]);
+        // piece `warp` of column 4 lane + j, at a place that differs between the sixteen lanes of a store's half warp
+        *reinterpret_cast<uint2*>(sh.turned + (lane * 4 + j) * 128 + ((warp ^ (lane & 15)) << 3)) = q;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = warp * 8 + i * 4 + (lane >> 3);
+        const int piece = lane & 7, turn = (c >> 2) & 15;
+        uint4 q = *reinterpret_cast<const uint4*>(sh.turned + c * 128 + ((((2 * piece) ^ turn) & ~1) << 3));
+        if (turn & 1) q = make_uint4(q.z, q.w, q.x, q.y);
+        const long long at = static_cast<long long>(tile_r) * 128 + piece * 16;
+        if (tile_c * 128 + c < a.cols && at < a.pitch_t)
+          *reinterpret_cast<uint4*>(a.codes_t + (static_cast<long long>(tile_c) * 128 + c) * a.pitch_t + at) = q;
+      }
     }
   }
 }
@@ -614,14 +694,162 @@ __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) rms_bwd_kernel(cons
   }
 }
 
+// The same pass with the rows brought into shared memory by bulk copies several batches ahead, for rows on 16-byte
+// boundaries.  A row belongs to `team` warps (8 NV values a thread), a batch is the `batch` rows that fit a CTA's eight or
+// sixteen; two CTAs of eight an SM cover one another's reductions (16384 x 4096 bf16: 119 us with direct loads).  The row is read from shared memory twice (for the sums, then for the gradient), so a thread keeps only the gain and its
+// partial sums, which the teams of a CTA add up at the end: one row of `part` a CTA.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+template <typename T, typename TG, int NV, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) rms_bwd_ring_kernel(const RmsBwdArgs a, int team, int batch, int stages, int* status) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ __align__(8) uint64_t full[8];
+  __shared__ float sums[2][WARPS];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int mine = warp / team;                              // this thread's team; rows of the batch behind the last one idle
+  const int G = team * 32, g = (warp % team) * 32 + lane;
+  const int C = a.cols;
+  const int t_bytes = C * static_cast<int>(sizeof(T)), g_bytes = C * static_cast<int>(sizeof(TG));
+  const int row_bytes = t_bytes + g_bytes + (a.gsum != nullptr ? t_bytes : 0);
+  const long long batches = (static_cast<long long>(a.rows) + batch - 1) / batch;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+    abort_word = 0;
+    fence_mbar_init();
+  }
+  grid_dependency_wait();
+  __syncthreads();
+  // one warp brings a batch: a lane per row and array
+  auto fetch = [&](long long b, int s) {
+    const int rows = static_cast<int>(min(static_cast<long long>(batch), a.rows - b * batch));
+    if (lane == 0) mbar_expect_tx(&full[s], static_cast<uint32_t>(rows * row_bytes));
+    __syncwarp();
+    for (int k = lane; k < rows * 3; k += 32) {
+      const long long row = b * batch + k / 3;
+      const uint32_t dst = smem_u32(ring) + static_cast<uint32_t>((s * batch + k / 3) * row_bytes);
+      if (k % 3 == 0) bulk_load(dst, static_cast<const T*>(a.t) + row * a.ldt, t_bytes, &full[s]);
+      else if (k % 3 == 1) bulk_load(dst + t_bytes, static_cast<const TG*>(a.g) + row * C, g_bytes, &full[s]);
+      else if (a.gsum != nullptr) bulk_load(dst + t_bytes + g_bytes, static_cast<const T*>(a.gsum) + row * C, t_bytes, &full[s]);
+    }
+  };
+  if (warp == 0)
+    for (int s = 0; s < stages; ++s) {
+      const long long b = blockIdx.x + static_cast<long long>(s) * gridDim.x;
+      if (b < batches) fetch(b, s);
+    }
+  float w[NV][8], dw[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    gain8<true>(a.gain, a.gain_type, (i * G + g) * 8, 1, C, w[i]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[i][e] = 0.f;
+  }
+  auto rstd_of = [&](long long b) {
+    const long long row = b * batch + mine;
+    return mine < batch && row < a.rows ? __ldg(a.rstd + row) : 0.f;
+  };
+  auto vec = [&](auto* p, float (&v)[8]) {
+    using E = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+    __align__(16) E raw[8];
+#pragma unroll
+    for (int k = 0; k < static_cast<int>(sizeof(E)) / 2; ++k) reinterpret_cast<uint4*>(raw)[k] = reinterpret_cast<const uint4*>(p)[k];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = to_f32<E>(raw[e]);
+  };
+  float r = rstd_of(blockIdx.x);
+  int s = 0, turn = 0;
+  uint32_t ph = 0;
+  for (long long b = blockIdx.x; b < batches; b += gridDim.x, turn ^= 1) {
+    const float r_next = rstd_of(b + gridDim.x);
+    mbar_wait(&full[s], ph, abort_flag, status, 8);
+    const long long row = b * batch + mine;
+    if (mine < batch && row < a.rows) {
+      const uint8_t* at = ring + (s * batch + mine) * row_bytes;
+      const T* ts = reinterpret_cast<const T*>(at);
+      const TG* gs = reinterpret_cast<const TG*>(at + t_bytes);
+      float dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * G + g) * 8;
+        if (c < C) {
+          float t[8], y[8];
+          vec(ts + c, t);
+          vec(gs + c, y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            dw[i][e] = fmaf(y[e], t[e] * r, dw[i][e]);
+            dot = fmaf(y[e] * w[i][e], t[e], dot);
+          }
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      if (team > 1) {
+        if (lane == 0) sums[turn][warp] = dot;
+        named_barrier(1 + mine, G);
+        dot = 0.f;
+        for (int k = 0; k < team; ++k) dot += sums[turn][mine * team + k];
+      }
+      const float k3 = r * r * (dot / static_cast<float>(C));
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * G + g) * 8;
+        if (c < C) {
+          float t[8], y[8], d[8];
+          vec(ts + c, t);
+          vec(gs + c, y);
+          if (a.gsum != nullptr) {
+            vec(reinterpret_cast<const T*>(at + t_bytes + g_bytes) + c, d);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[e] = fmaf(r, y[e] * w[i][e] - t[e] * k3, d[e]);
+          store8<T, true>(static_cast<T*>(a.dx) + row * C, c, 1, C, d);
+        }
+      }
+    }
+    r = r_next;
+    __syncthreads();                          // the batch has been read
+    const long long later = b + static_cast<long long>(stages) * gridDim.x;
+    if (warp == 0 && later < batches) fetch(later, s);
+    if (++s == stages) { s = 0; ph ^= 1u; }
+  }
+  if (*abort_flag) {                          // a wait gave up: let the copies already issued arrive before the CTA ends
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  if (a.part != nullptr) {
+    __syncthreads();
+    float* sum = reinterpret_cast<float*>(ring);           // [batch][C]
+    if (mine < batch) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) store8<float, true>(sum + static_cast<long long>(mine) * C, (i * G + g) * 8, 1, C, dw[i]);
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < C; c += WARPS * 32) {
+      float v = 0.f;
+      for (int k = 0; k < batch; ++k) v += sum[k * C + c];
+      a.part[static_cast<long long>(blockIdx.x) * C + c] = v;
+    }
+  }
+}
+
 // ---------------------------------------------------------------- dispatch
 // Launch that may begin while earlier work of the stream still runs: every kernel here calls grid_dependency_wait() before
 // it touches memory, so only its launch and set-up overlap (about 2 us a launch in a chain of short kernels).
 template <typename Kernel, typename Args, typename... More>
-static cudaError_t launch_chained(Kernel kernel, dim3 grid, dim3 block, cudaStream_t stream, const Args& first, More... more) {
+static cudaError_t launch_chained(Kernel kernel, dim3 grid, dim3 block, cudaStream_t stream, int smem, const Args& first, More... more) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -642,16 +870,47 @@ template <typename T, bool VEC, bool CODES>
 static int launch_rms_fwd(const RmsArgs& a, int sm_count, cudaStream_t st) {
   const int warps = (a.rows + 7) / 8;
   if (a.rows < sm_count && a.cols > 256 && a.cols <= 8192)
-    launch_chained(rms_fwd_kernel<T, 1, VEC, false, CODES, 1024>, dim3(a.rows), dim3(rms_threads(a.cols, 8)), st, a);
-  else if (a.cols <= 512) launch_chained(rms_fwd_kernel<T, 2, VEC, true, CODES, 256>, dim3(warps), dim3(256), st, a);
-  else if (a.cols <= 1024) launch_chained(rms_fwd_kernel<T, 4, VEC, true, CODES, 256>, dim3(warps), dim3(256), st, a);
-  else if (a.cols <= 16384) launch_chained(rms_fwd_kernel<T, 4, VEC, false, CODES, 512>, dim3(a.rows), dim3(rms_threads(a.cols, 32)), st, a);
-  else launch_chained(rms_fwd_kernel<T, 4, VEC, false, CODES, 1024>, dim3(a.rows), dim3(rms_threads(a.cols, 32)), st, a);
+    launch_chained(rms_fwd_kernel<T, 1, VEC, false, CODES, 1024>, dim3(a.rows), dim3(rms_threads(a.cols, 8)), st, 0, a);
+  else if (a.cols <= 512) launch_chained(rms_fwd_kernel<T, 2, VEC, true, CODES, 256>, dim3(warps), dim3(256), st, 0, a);
+  else if (a.cols <= 1024) launch_chained(rms_fwd_kernel<T, 4, VEC, true, CODES, 256>, dim3(warps), dim3(256), st, 0, a);
+  else if (a.cols <= 16384) launch_chained(rms_fwd_kernel<T, 4, VEC, false, CODES, 512>, dim3(a.rows), dim3(rms_threads(a.cols, 32)), st, 0, a);
+  else launch_chained(rms_fwd_kernel<T, 4, VEC, false, CODES, 1024>, dim3(a.rows), dim3(rms_threads(a.cols, 32)), st, 0, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
-// Backward: a thread holds three arrays (row, gradient, partial sums of the gain) and the next row, 16 values of each up to
-// 8192 columns and 32 beyond; rows beyond 16384 take 1024 threads and spill.
+// How the backward pass cuts its work.  Ring: two CTAs of eight warps an SM where two batches of a row fit each (16-bit rows
+// up to 8192), one of sixteen otherwise; NV is the one of 2, 3, 4 that leaves the fewest threads idle.  fp32 rows beyond 8192
+// and rows beyond 16384 do not fit.  Otherwise (and for rows that are not on 16-byte boundaries) direct loads: a thread holds
+// row, gradient, partial sums and the next row, 16 values of each up to 8192 columns and 32 beyond; rows beyond 16384 spill.
+struct RmsBwdPlan {
+  int nv, warps, team, batch, stages, ring_bytes, ctas;    // nv = 0: direct loads
+};
+static inline RmsBwdPlan rms_bwd_ring(int rows, int cols, int bytes_per_value, int sm_count) {
+  RmsBwdPlan best{};
+  for (int warps = 8; warps <= 16 && best.nv == 0; warps += 8) {
+    const int most = sm_count * (16 / warps);
+    int used = 0;
+    for (int nv = 2; nv <= 4; ++nv) {
+      const int team = (cols + 256 * nv - 1) / (256 * nv);
+      if (team > warps) continue;
+      // few rows: smaller batches, so that every CTA has one
+      int batch = warps / team;
+      const int fair = (rows + most - 1) / most;
+      if (batch > fair) batch = fair;
+      const int share = static_cast<int>(1000LL * cols * (warps / team) / (warps * 256 * nv));
+      const int stage = batch * cols * bytes_per_value;
+      int stages = (warps == 8 ? 104 : 208) * 1024 / stage;
+      if (stages > 6) stages = 6;
+      if (stages < 2 || share <= used) continue;
+      const int need = batch * cols * 4;         // the partial sums of the teams, at the end
+      const long long batches = (static_cast<long long>(rows) + batch - 1) / batch;
+      used = share;
+      best = RmsBwdPlan{nv, warps, team, batch, stages, stages * stage > need ? stages * stage : need,
+                        static_cast<int>(batches < most ? batches : most)};
+    }
+  }
+  return best;
+}
 static inline bool rms_bwd_by_warp(int cols) { return cols <= 512; }
 static inline int rms_bwd_threads(int cols) {
   return rms_bwd_by_warp(cols) ? 256 : rms_threads(cols, cols <= 8192 ? 16 : 32);
@@ -663,39 +922,78 @@ static inline int rms_bwd_ctas(int rows, int cols, int sm_count) {
   const long long most = static_cast<long long>(sm_count) * resident;
   return static_cast<int>(want < most ? want : most);
 }
+// Wide loads are possible: the ring's condition too.
+static inline bool rms_bwd_wide(const JbRmsBwd* q) {
+  const long long size = q->type == 0 ? 4 : 2;
+  return q->cols % 8 == 0 && (q->ldt * size) % 16 == 0 && aligned16(q->t) && aligned16(q->g) && aligned16(q->gsum) &&
+         aligned16(q->gain) && aligned16(q->dx);
+}
+static inline int rms_bwd_bytes(const JbRmsBwd* q) {
+  const int size = q->type == 0 ? 4 : 2;
+  return size + (q->g_f32 ? 4 : size) + (q->gsum != nullptr ? size : 0);
+}
 
-template <typename T, typename TG, bool VEC>
-static int launch_rms_bwd(const RmsBwdArgs& a, int sm_count, cudaStream_t st) {
+template <typename T, typename TG>
+static int launch_rms_bwd(const RmsBwdArgs& a, bool wide, const RmsBwdPlan& plan, int sm_count, int* status, cudaStream_t st) {
+  if (plan.nv != 0) {
+    auto go = [&](auto kernel) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, plan.ring_bytes) != cudaSuccess) return -3;
+      return launch_chained(kernel, dim3(plan.ctas), dim3(plan.warps * 32), st, plan.ring_bytes, a, plan.team, plan.batch, plan.stages, status) == cudaSuccess ? 0 : -4;
+    };
+    if (plan.warps == 8) {
+      if (plan.nv == 2) return go(rms_bwd_ring_kernel<T, TG, 2, 8>);
+      if (plan.nv == 3) return go(rms_bwd_ring_kernel<T, TG, 3, 8>);
+      return go(rms_bwd_ring_kernel<T, TG, 4, 8>);
+    }
+    if (plan.nv == 2) return go(rms_bwd_ring_kernel<T, TG, 2, 16>);
+    if (plan.nv == 3) return go(rms_bwd_ring_kernel<T, TG, 3, 16>);
+    return go(rms_bwd_ring_kernel<T, TG, 4, 16>);
+  }
   const int grid = rms_bwd_ctas(a.rows, a.cols, sm_count), threads = rms_bwd_threads(a.cols);
-  if (rms_bwd_by_warp(a.cols)) launch_chained(rms_bwd_kernel<T, TG, 2, VEC, true, 256>, dim3(grid), dim3(threads), st, a);
-  else if (threads <= 256 && a.cols <= 8192) launch_chained(rms_bwd_kernel<T, TG, 2, VEC, false, 256>, dim3(grid), dim3(threads), st, a);
-  else if (a.cols <= 8192) launch_chained(rms_bwd_kernel<T, TG, 2, VEC, false, 512>, dim3(grid), dim3(threads), st, a);
-  else if (a.cols <= 16384) launch_chained(rms_bwd_kernel<T, TG, 4, VEC, false, 512>, dim3(grid), dim3(threads), st, a);
-  else launch_chained(rms_bwd_kernel<T, TG, 4, VEC, false, 1024>, dim3(grid), dim3(threads), st, a);
+#define JB_BWD(NV, VEC, WARP, MOST) launch_chained(rms_bwd_kernel<T, TG, NV, VEC, WARP, MOST>, dim3(grid), dim3(threads), st, 0, a)
+  if (a.cols > 16384) {
+    if (wide) JB_BWD(4, true, false, 1024);
+    else JB_BWD(4, false, false, 1024);
+  } else if (a.cols > 8192) {
+    if (wide) JB_BWD(4, true, false, 512);
+    else JB_BWD(4, false, false, 512);
+  } else if (rms_bwd_by_warp(a.cols)) {          // the ring takes every wide case up to here
+    JB_BWD(2, false, true, 256);
+  } else if (threads <= 256) {
+    JB_BWD(2, false, false, 256);
+  } else {
+    JB_BWD(2, false, false, 512);
+  }
+#undef JB_BWD
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
 template <typename T>
-static int launch_quant(const QuantArgs& a, bool tiles, cudaStream_t st) {
+static int launch_quant(const QuantArgs& a, bool tiles, int sm_count, cudaStream_t st) {
   const long long size = static_cast<long long>(sizeof(T));
   const int kblocks = (a.cols + 127) / 128, rblocks = (a.rows + 127) / 128;
   if (tiles) {
-    const bool vec = a.cols % 4 == 0 && (a.ldx * size) % (4 * size) == 0 && (reinterpret_cast<uintptr_t>(a.x) & (4 * size - 1)) == 0;
-    if (kblocks > 65535) return -1;
-    const dim3 grid(rblocks, kblocks);
-    if (a.rstd != nullptr) {
-      if (vec) launch_chained(quant_tile_kernel<T, true, true>, dim3(grid), dim3(512), st, a);
-      else launch_chained(quant_tile_kernel<T, false, true>, dim3(grid), dim3(512), st, a);
-    } else {
-      if (vec) launch_chained(quant_tile_kernel<T, true, false>, dim3(grid), dim3(512), st, a);
-      else launch_chained(quant_tile_kernel<T, false, false>, dim3(grid), dim3(512), st, a);
-    }
+    const bool vec = (a.cols * size) % 16 == 0 && (a.ldx * size) % 16 == 0 && aligned16(a.x);
+    const long long n = static_cast<long long>(rblocks) * kblocks;
+    if (n > 0x7fffffffLL - 1024) return -1;
+    auto go = [&](auto kernel, int smem) {
+      const long long most = 2LL * sm_count;          // two CTAs an SM
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -3;
+      return launch_chained(kernel, dim3(static_cast<unsigned>(n < most ? n : most)), dim3(512), st, smem, a, rblocks, static_cast<int>(n)) == cudaSuccess ? 0 : -4;
+    };
+    constexpr int FAST = sizeof(T) == 2 ? QT_AHEAD : QT_WIDE;
+#define JB_TILE(NORM)                                                                                   \
+  return vec ? go(quant_tile_kernel<T, FAST, NORM>, quant_tile_smem<T, FAST>())                         \
+             : go(quant_tile_kernel<T, QT_PLAIN, NORM>, quant_tile_smem<T, QT_PLAIN>());
+    if (a.rstd != nullptr) { JB_TILE(true) }
+    JB_TILE(false)
+#undef JB_TILE
   } else {
     const bool vec = a.cols % 8 == 0 && (a.ldx * size) % 16 == 0 && aligned16(a.x);
     if ((kblocks + 7) / 8 > 65535) return -1;
     const dim3 grid((a.rows + 31) / 32, (kblocks + 7) / 8);
-    if (vec) launch_chained(quant_rows_kernel<T, true>, dim3(grid), dim3(256), st, a);
-    else launch_chained(quant_rows_kernel<T, false>, dim3(grid), dim3(256), st, a);
+    if (vec) launch_chained(quant_rows_kernel<T, true>, dim3(grid), dim3(256), st, 0, a);
+    else launch_chained(quant_rows_kernel<T, false>, dim3(grid), dim3(256), st, 0, a);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
@@ -705,7 +1003,7 @@ static int launch_quant(const QuantArgs& a, bool tiles, cudaStream_t st) {
 // Codes and scales of x (times rstd and gain) by rows, by columns (transposed), both, or in squares of 128 x 128 (both
 // layouts share the scales).  Pitches are multiples of 16; bytes between the last value and the pitch are written as 0
 // within the last 8 (transposed: 16) bytes only.
-extern "C" int jb_quantize(const JbQuant* q, void* stream) {
+extern "C" int jb_quantize(const JbQuant* q, int sm_count, void* stream) {
   using namespace jb;
   if (q == nullptr || q->rows < 1 || q->cols < 1 || (q->codes == nullptr && q->codes_t == nullptr)) return -1;
   if (q->codes != nullptr && ((q->pitch & 15) || !aligned16(q->codes) || q->pitch < q->cols)) return -1;
@@ -718,17 +1016,19 @@ extern "C" int jb_quantize(const JbQuant* q, void* stream) {
   a.scales_t = static_cast<uint8_t*>(q->scales_t); a.scale_t_row = q->scale_t_row; a.scale_t_k = q->scale_t_k;
   a.rstd = static_cast<const float*>(q->rstd); a.gain = q->gain; a.gain_type = q->gain_type;
   a.colsum = static_cast<float*>(q->colsum); a.square = q->square;
-  const bool tiles = q->square || q->codes_t != nullptr || q->rstd != nullptr || q->colsum != nullptr;
+  // rows alone: a warp per 32 rows of one block column is quick for few rows, tiles for many (8192 x 11008 bf16: 94 us
+  // against 56)
+  const bool tiles = q->square || q->codes_t != nullptr || q->rstd != nullptr || q->colsum != nullptr || q->rows >= 128;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (q->type == 0) return launch_quant<float>(a, tiles, st);
-  if (q->type == 1) return launch_quant<__nv_bfloat16>(a, tiles, st);
-  if (q->type == 2) return launch_quant<__half>(a, tiles, st);
+  if (q->type == 0) return launch_quant<float>(a, tiles, sm_count, st);
+  if (q->type == 1) return launch_quant<__nv_bfloat16>(a, tiles, sm_count, st);
+  if (q->type == 2) return launch_quant<__half>(a, tiles, sm_count, st);
   return -1;
 }
 
 extern "C" int jb_column_sum(const float* part, int P, int C, void* out, int out_type, void* stream) {
   if (P < 1 || C < 1) return -1;
-  return jb::launch_chained(jb::column_sum_kernel, dim3((C + 31) / 32), dim3(32, 32), static_cast<cudaStream_t>(stream), part, P, C, out, out_type) == cudaSuccess ? 0 : -4;
+  return jb::launch_chained(jb::column_sum_kernel, dim3((C + 31) / 32), dim3(32, 32), static_cast<cudaStream_t>(stream), 0, part, P, C, out, out_type) == cudaSuccess ? 0 : -4;
 }
 
 // Longest row that the kernels keep in registers.
@@ -758,23 +1058,25 @@ extern "C" int jb_rms_norm_fwd(const JbRms* q, int sm_count, void* stream) {
 #undef JB_RMS
 }
 
-// Rows of the gain's partial sums that jb_rms_norm_bwd writes.
-extern "C" int jb_rms_bwd_parts(int rows, int cols, int sm_count) {
-  return jb::rms_bwd_ctas(rows, cols, sm_count) * (jb::rms_bwd_by_warp(cols) ? 8 : 1);
+// Rows of the gain's partial sums that jb_rms_norm_bwd writes for these arguments.
+extern "C" int jb_rms_bwd_parts(const JbRmsBwd* q, int sm_count) {
+  using namespace jb;
+  const RmsBwdPlan plan = rms_bwd_wide(q) ? rms_bwd_ring(q->rows, q->cols, rms_bwd_bytes(q), sm_count) : RmsBwdPlan{};
+  if (plan.nv != 0) return plan.ctas;
+  return rms_bwd_ctas(q->rows, q->cols, sm_count) * (rms_bwd_by_warp(q->cols) ? 8 : 1);
 }
 
-extern "C" int jb_rms_norm_bwd(const JbRmsBwd* q, int sm_count, void* stream) {
+extern "C" int jb_rms_norm_bwd(const JbRmsBwd* q, int sm_count, int* status, void* stream) {
   using namespace jb;
   if (q == nullptr || q->rows < 1 || q->cols < 1 || q->cols > jb_rms_max_cols() || q->type < 0 || q->type > 2) return -1;
   RmsBwdArgs a{};
   a.t = q->t; a.ldt = q->ldt; a.g = q->g; a.gsum = q->gsum;
   a.rstd = static_cast<const float*>(q->rstd); a.gain = q->gain; a.gain_type = q->gain_type; a.rows = q->rows; a.cols = q->cols;
   a.dx = q->dx; a.part = static_cast<float*>(q->part);
-  const long long size = q->type == 0 ? 4 : 2;
-  const bool vec = q->cols % 8 == 0 && (q->ldt * size) % 16 == 0 && aligned16(q->t) && aligned16(q->g) && aligned16(q->gsum) &&
-                   aligned16(q->gain) && aligned16(q->dx) && aligned16(q->part);
+  const bool wide = rms_bwd_wide(q);
+  const RmsBwdPlan plan = wide ? rms_bwd_ring(q->rows, q->cols, rms_bwd_bytes(q), sm_count) : RmsBwdPlan{};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define JB_RMS(T, TG) return vec ? launch_rms_bwd<T, TG, true>(a, sm_count, st) : launch_rms_bwd<T, TG, false>(a, sm_count, st);
+#define JB_RMS(T, TG) return launch_rms_bwd<T, TG>(a, wide && aligned16(q->part), plan, sm_count, status, st);
   if (q->type == 0) { JB_RMS(float, float) }
   if (q->type == 1) {
     if (q->g_f32) { JB_RMS(__nv_bfloat16, float) }

@@ -67,6 +67,14 @@ int checked(int64_t n) {
 }
 int64_t pitch_of(int64_t n) { return (n + 15) / 16 * 16; }
 
+std::array<Tensor, 64> status_words;                 // per device, set by Python when it first meets one
+void set_status(int64_t device, const Tensor& word) { status_words.at(device) = word; }
+const Tensor& status_of(const Tensor& t) {
+  const Tensor& w = status_words.at(t.device().index());
+  TORCH_CHECK(w.defined(), "no status word for device ", t.device().index());
+  return w;
+}
+
 // A tensor as rows of its last axis, `ld` elements apart; copied only if its strides do not allow that.
 struct Rows {
   Tensor t;
@@ -187,7 +195,7 @@ Quantized quantize(const Tensor& input, bool square, bool want_rows, bool want_c
     part = empty({rb, x.cols}, at::kFloat, x.t);
     q.colsum = part.data_ptr();
   }
-  done(api.quantize(&q, stream_of(x.t)), "quantize");
+  done(api.quantize(&q, sm_count(x.t), stream_of(x.t)), "quantize");
   if (sum_type >= 0) {
     out.sums = empty({x.cols}, scalar_of(sum_type), x.t);
     done(api.column_sum(part.const_data_ptr<float>(), checked(rb), q.cols, out.sums.data_ptr(), sum_type, stream_of(x.t)), "column_sum");
@@ -291,10 +299,10 @@ std::pair<Tensor, Tensor> rms_backward(const Tensor& sum, const Tensor& gain, co
   q.dx = dx.data_ptr();
   const int sm = sm_count(sum);
   if (want_gain) {
-    part = empty({api.rms_bwd_parts(q.rows, q.cols, sm), t.cols}, at::kFloat, sum);
+    part = empty({api.rms_bwd_parts(&q, sm), t.cols}, at::kFloat, sum);
     q.part = part.data_ptr();
   }
-  done(api.rms_bwd(&q, sm, stream_of(sum)), "rms_norm_bwd");
+  done(api.rms_bwd(&q, sm, status_of(sum).data_ptr<int>(), stream_of(sum)), "rms_norm_bwd");
   if (want_gain) {
     dgain = empty({t.cols}, gain.scalar_type(), sum);
     done(api.column_sum(part.const_data_ptr<float>(), checked(part.size(0)), q.cols, dgain.data_ptr(), q.gain_type, stream_of(sum)),
@@ -548,14 +556,6 @@ int autocast_type(const Tensor& x) {
   if (!at::autocast::is_autocast_enabled(at::kCUDA)) return type_of(x.scalar_type());
   const at::ScalarType t = at::autocast::get_autocast_dtype(at::kCUDA);
   return t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : type_of(x.scalar_type());
-}
-
-std::array<Tensor, 64> status_words;                 // per device, set by Python when it first meets one
-void set_status(int64_t device, const Tensor& word) { status_words.at(device) = word; }
-const Tensor& status_of(const Tensor& t) {
-  const Tensor& w = status_words.at(t.device().index());
-  TORCH_CHECK(w.defined(), "no status word for device ", t.device().index());
-  return w;
 }
 
 py::object py_quantize(const Tensor& x, bool square, bool rows, bool cols, const Optional& rstd, const Optional& gain, int sum_type) {

@@ -103,7 +103,7 @@ def prepared_linear(x: torch.Tensor, w: Any, b: torch.Tensor | None) -> torch.Te
 @_lib.traced("jb.rms_norm")
 def rms_norm(x: torch.Tensor, gain: torch.Tensor | None, residual: torch.Tensor | None, eps: float) -> tuple | None:
     """Differentiable ``(y, x + residual)``."""
-    return _answer("rms_norm", (_native or native()).rms_norm(x, gain, residual, eps))
+    return _answer("rms_norm", _on(x).rms_norm(x, gain, residual, eps))
 
 
 @_lib.traced("jb.rms_norm_quantize")
