@@ -149,9 +149,13 @@ struct SgSmem {
   static constexpr int TILE_BYTES = P_BYTES + Q_ROWS * 128;        // multiples of 1024: swizzled operands
   static constexpr int SF_BYTES = 512 * (1 + Q_ATOMS);             // scale words of four k-blocks
   static constexpr int SF_SLOTS = 3;
-  static constexpr int STAGES = TILE_BYTES >= 49152 ? 4 : TILE_BYTES >= 32768 ? (JOIN ? 4 : 6) : JOIN && BQ >= 64 ? 6 : 8;
-  static constexpr int ACCS = BQ >= 256 ? 1 : 2;
-  static constexpr int SF_OFFSET = STAGES * TILE_BYTES;
+  // Narrow tiles are bound by the hand-overs and by the latency of dependent products (16 columns: 90 cycles a product, of
+  // which a k-block has four): two k-blocks a stage, and the products take turns between two accumulators.
+  static constexpr int KPS = BQ <= 64 ? 2 : 1;                     // k-blocks a stage
+  static constexpr bool DUAL = BQ <= 64;
+  static constexpr int STAGES = TILE_BYTES >= 49152 ? 4 : TILE_BYTES >= 32768 ? (JOIN ? 4 : 6) : BQ >= 64 ? 3 : 4;
+  static constexpr int ACCS = BQ >= 256 || DUAL ? 1 : 2;           // tiles in TMEM
+  static constexpr int SF_OFFSET = STAGES * KPS * TILE_BYTES;
   static constexpr int OUT_OFFSET = SF_OFFSET + SF_SLOTS * SF_BYTES;
   // plain: 32 rows x 64 bytes per draining warp; JOIN: the parts of BQ / split columns from each CTA
   static constexpr int OUT_BYTES = JOIN ? (BQ * SG_PITCH * 4 + 15) / 16 * 16 : SG_EPI_WARPS * 2048;
@@ -160,7 +164,7 @@ struct SgSmem {
   static constexpr int TOTAL = BAR_OFFSET + 256 + 1024;
   static_assert(TOTAL <= 227 * 1024, "shared memory of one CTA");
   static_assert(BARS * 8 + 8 <= 256, "barriers");
-  static constexpr int SF_COL = ACCS * BQ < 32 ? 32 : ACCS * BQ;   // first TMEM column of the scales
+  static constexpr int SF_COL = (DUAL ? 2 : ACCS) * BQ;            // first TMEM column of the scales
   static constexpr int SF_COLS = 4 * (1 + Q_ATOMS);
   static_assert(SF_COL + SF_SLOTS * SF_COLS <= 512, "TMEM columns");
 };
@@ -208,7 +212,7 @@ template <int BQ, bool PAIR, bool SWAP, bool JOIN>
 __global__ void __launch_bounds__(SG_THREADS, 1)
 scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ, const ScaledGemmArgs a,
                    int* status) {
-  static_assert(!(PAIR && JOIN) && (JOIN || !SWAP), "forms");
+  static_assert(!(PAIR && JOIN) && (JOIN || !SWAP) && SWAP == (BQ <= 64), "forms");
   using S = SgSmem<BQ, PAIR, JOIN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -246,14 +250,20 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constan
   const int q_off = PAIR ? static_cast<int>(rank) * S::Q_ROWS : 0;
   constexpr int P_TILE = PAIR ? 2 * SG_BP : SG_BP;
 
-  auto load_stage = [&](int s, int kb, int tp, int tq) {
-    uint8_t* dst = smem + s * S::TILE_BYTES;
-    mbar_expect_tx(&full[s], S::TILE_BYTES);
-    tma_load_2d(dst, &tmP, &full[s], kb * 128, tp * P_TILE + p_off);
-    tma_load_2d(dst + S::P_BYTES, &tmQ, &full[s], kb * 128, tq * BQ + q_off);
+  auto load_stage = [&](int s, int kb, int tp, int tq) {          // k-blocks kb .. kb + KPS - 1 below kb1
+    const int n = min(S::KPS, kb1 - kb);
+    mbar_expect_tx(&full[s], n * S::TILE_BYTES);
+#pragma unroll
+    for (int j = 0; j < S::KPS; ++j) {
+      if (j < n) {
+        uint8_t* dst = smem + (s * S::KPS + j) * S::TILE_BYTES;
+        tma_load_2d(dst, &tmP, &full[s], (kb + j) * 128, tp * P_TILE + p_off);
+        tma_load_2d(dst + S::P_BYTES, &tmQ, &full[s], (kb + j) * 128, tq * BQ + q_off);
+      }
+    }
   };
 
-  int early = 0;             // k-blocks of the first tile whose loads are issued before the CTA has met
+  int early = 0;             // stages of the first tile whose loads are issued before the CTA has met
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
       mbar_init(&full[s], PAIR && rank == 0 ? 2 : 1);
@@ -273,7 +283,7 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constan
     if (first_tile < tiles) {
       int tp, tq;
       sg_tile(first_tile, a.tiles_p, a.tiles_q, tp, tq);
-      for (; early < S::STAGES && kb0 + early < kb1; ++early) load_stage(early, kb0 + early, tp, tq);
+      for (; early < S::STAGES && kb0 + early * S::KPS < kb1; ++early) load_stage(early, kb0 + early * S::KPS, tp, tq);
     }
   }
   if (warp == 1) {
@@ -306,7 +316,7 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constan
       for (int t = first_tile; t < tiles && ok; t += step) {
         int tp, tq;
         sg_tile(t, a.tiles_p, a.tiles_q, tp, tq);
-        for (int kb = kb0 + skip; kb < kb1; ++kb) {
+        for (int kb = kb0 + skip * S::KPS; kb < kb1; kb += S::KPS) {
           ok = mbar_wait(&empty[s], ph ^ 1u, abort_flag, status, 1);
           if (!ok) break;
           load_stage(s, kb, tp, tq);
@@ -393,36 +403,45 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constan
         mbar_wait(&acc_empty[as], aph ^ 1u, abort_flag, status, 3);
         tc_fence_after_sync();
         const uint32_t d = tmem + static_cast<uint32_t>(as * BQ);
-        for (int kb = c0; kb < c1; ++kb) {
-          mbar_wait(&full[s], ph, abort_flag, status, 4);
-          tc_fence_after_sync();
-          const uint64_t pd = desc_advance(pd0, static_cast<uint32_t>(s * S::TILE_BYTES));
-          const uint64_t qd = desc_advance(qd0, static_cast<uint32_t>(s * S::TILE_BYTES));
-          const int byte = kb & 3;
+        // One scale word (four k-blocks) a turn, unrolled: the issuing warp is a single thread's chain of instructions, and for
+        // narrow tiles that chain, not the products, was the time of a k-block.
+        for (int kb4 = c0; kb4 < c1; kb4 += 4) {
+          mbar_wait(&sf_full[f], fph, abort_flag, status, 7);
           const uint32_t sfp = tmem + S::SF_COL + static_cast<uint32_t>(f * S::SF_COLS);
           const uint32_t sfq = sfp + 4;
-          if (byte == 0) {
-            mbar_wait(&sf_full[f], fph, abort_flag, status, 7);
-            tc_fence_after_sync();
-          }
-          const bool last_of_word = byte == 3 || kb + 1 == kb1;
-          if (elect_one()) {
-            if (byte == 0) {
-              const uint64_t sd = desc_advance(sd0, static_cast<uint32_t>(f * S::SF_BYTES));
-              tmem_cp_scales<PAIR>(sfp, sd);
+          const uint64_t sd = desc_advance(sd0, static_cast<uint32_t>(f * S::SF_BYTES));
+          const int left = c1 - kb4;                 // k-blocks of this word
 #pragma unroll
-              for (int g = 0; g < S::Q_ATOMS; ++g) tmem_cp_scales<PAIR>(sfq + 4 * g, desc_advance(sd, 512 * (1 + g)));
+          for (int j = 0; j < 4; j += S::KPS) {
+            if (j < left) {
+              mbar_wait(&full[s], ph, abort_flag, status, 4);
+              tc_fence_after_sync();
+              const uint64_t pd = desc_advance(pd0, static_cast<uint32_t>(s * S::KPS * S::TILE_BYTES));
+              const uint64_t qd = desc_advance(qd0, static_cast<uint32_t>(s * S::KPS * S::TILE_BYTES));
+              if (elect_one()) {
+                if (j == 0) {
+                  tmem_cp_scales<PAIR>(sfp, sd);
+#pragma unroll
+                  for (int g = 0; g < S::Q_ATOMS; ++g) tmem_cp_scales<PAIR>(sfq + 4 * g, desc_advance(sd, 512 * (1 + g)));
+                }
+#pragma unroll
+                for (int i = 0; i < S::KPS; ++i) {
+                  if (i == 0 || j + i < left) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)          // 32 codes = 32 bytes of the swizzled row
+                      umma_mxf8<PAIR>(d + (S::DUAL ? (k & 1) * BQ : 0), desc_advance(pd, i * S::TILE_BYTES + k * 32),
+                                      desc_advance(qd, i * S::TILE_BYTES + k * 32), make_idesc_mxf8(P_TILE, BQ, j + i), sfp, sfq,
+                                      (kb4 > c0 || j + i > 0 || k > (S::DUAL ? 1 : 0)) ? 1u : 0u);
+                  }
+                }
+                sg_commit<PAIR>(&empty[s]);
+                if (j + S::KPS >= left || j + S::KPS >= 4) sg_commit<PAIR>(&sf_empty[f]);
+              }
+              __syncwarp();
+              if (++s == S::STAGES) { s = 0; ph ^= 1u; }
             }
-            const uint32_t idesc = make_idesc_mxf8(P_TILE, BQ, 0) | static_cast<uint32_t>(byte << 4) | (static_cast<uint32_t>(byte) << 29);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)          // 32 codes = 32 bytes of the swizzled row
-              umma_mxf8<PAIR>(d, desc_advance(pd, k * 32), desc_advance(qd, k * 32), idesc, sfp, sfq, (kb > c0 || k != 0) ? 1u : 0u);
-            if (last_of_word) sg_commit<PAIR>(&sf_empty[f]);
-            sg_commit<PAIR>(&empty[s]);
           }
-          __syncwarp();
-          if (last_of_word && ++f == S::SF_SLOTS) { f = 0; fph ^= 1u; }
-          if (++s == S::STAGES) { s = 0; ph ^= 1u; }
+          if (++f == S::SF_SLOTS) { f = 0; fph ^= 1u; }
         }
         if (elect_one()) sg_commit<PAIR>(&acc_full[as]);
         __syncwarp();
@@ -459,6 +478,16 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constan
             for (int j = 0; j < GROUP; ++j) {
               asm volatile("" : "+r"(raw[j]));          // no use above the wait
               acc[c + j] += __uint_as_float(raw[j]);
+            }
+            if constexpr (S::DUAL) {
+              if constexpr (GROUP == 32) tmem_ld_32x32(taddr + BQ + c, raw);
+              else tmem_ld_32x16(taddr + BQ + c, raw);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < GROUP; ++j) {
+                asm volatile("" : "+r"(raw[j]));
+                acc[c + j] += __uint_as_float(raw[j]);
+              }
             }
           }
         }
@@ -708,9 +737,21 @@ extern "C" int jb_scaled_gemm(const JbScaledOperand* a, const JbScaledOperand* b
 #define JB_SG(BQ, PAIR) return launch_scaled_gemm<BQ, PAIR, false, false>(a->codes, a->pitch, b->codes, b->pitch, K, g, 1, sm_count, status, st)
   if (M <= 64) {
     g.p = ob; g.q = oa;
+    // How many CTAs share a tile: the one of 1, 2, 4, 8 with the least of (k-blocks of a CTA, 0.17 us each, or reading the
+    // weight at 6.5 TB/s) and the meeting of the parts (2 us).  Measured, one token: 1024 x 4096 takes 9.8 us whole and 6.2 us
+    // in eight parts, 8192 x 4096 10.1 us whole and 10.5 us in two.
     const int tiles = (N + 127) / 128;
+    const float memory = static_cast<float>(N) * static_cast<float>(K) / 6.5e6f;
     int split = 1;
-    while (split < 8 && tiles * split * 2 <= sm_count && g.kblocks >= split * 8) split *= 2;
+    float least = 0.f;
+    for (int k = 1; k <= 8 && tiles * k <= (k == 1 ? tiles : sm_count) && g.kblocks >= 4 * k; k *= 2) {
+      const float own = 0.17f * g.kblocks / k;
+      const float cost = (own > memory ? own : memory) + (k > 1 ? 2.f : 0.f);
+      if (k == 1 || cost < least) {
+        least = cost;
+        split = k;
+      }
+    }
     if (M <= 16) return launch_scaled_gemm<16, false, true, true>(b->codes, b->pitch, a->codes, a->pitch, K, g, split, sm_count, status, st);
     if (M <= 32) return launch_scaled_gemm<32, false, true, true>(b->codes, b->pitch, a->codes, a->pitch, K, g, split, sm_count, status, st);
     return launch_scaled_gemm<64, false, true, true>(b->codes, b->pitch, a->codes, a->pitch, K, g, split, sm_count, status, st);

@@ -225,7 +225,7 @@ constexpr int quant_tile_smem() { return QT_SHARED + (MODE == QT_AHEAD ? 2 * 128
 // memory, eight bytes of a column at a time.  A CTA takes tiles in steps of the grid; of 16-bit values it has the next tile
 // copied into shared memory while it works on the present one (8192 x 11008 bf16, both layouts: 134 us with loads, which
 // the warps waited for half of the time).  Two fp32 tiles ahead would leave room for one CTA an SM, which is slower than
-// loads (11001 x 4100: 48 us against 39).
+// loads (11001 x 4100: 48 us against 42).
 template <typename T, int MODE, bool NORM>
 __global__ void __launch_bounds__(512, 2) quant_tile_kernel(const QuantArgs a, int tiles_r, int tiles) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -976,12 +976,13 @@ static int launch_quant(const QuantArgs& a, bool tiles, int sm_count, cudaStream
     const bool vec = (a.cols * size) % 16 == 0 && (a.ldx * size) % 16 == 0 && aligned16(a.x);
     const long long n = static_cast<long long>(rblocks) * kblocks;
     if (n > 0x7fffffffLL - 1024) return -1;
+    constexpr int FAST = sizeof(T) == 2 ? QT_AHEAD : QT_WIDE;
     auto go = [&](auto kernel, int smem) {
-      const long long most = 2LL * sm_count;          // two CTAs an SM
+      // two CTAs an SM where the next tile is copied ahead; without that a CTA a tile
+      const long long most = vec && FAST == QT_AHEAD ? 2LL * sm_count : n;
       if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -3;
       return launch_chained(kernel, dim3(static_cast<unsigned>(n < most ? n : most)), dim3(512), st, smem, a, rblocks, static_cast<int>(n)) == cudaSuccess ? 0 : -4;
     };
-    constexpr int FAST = sizeof(T) == 2 ? QT_AHEAD : QT_WIDE;
 #define JB_TILE(NORM)                                                                                   \
   return vec ? go(quant_tile_kernel<T, FAST, NORM>, quant_tile_smem<T, FAST>())                         \
              : go(quant_tile_kernel<T, QT_PLAIN, NORM>, quant_tile_smem<T, QT_PLAIN>());
