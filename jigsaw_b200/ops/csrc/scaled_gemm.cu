@@ -159,7 +159,9 @@ struct SgSmem {
   static constexpr int OUT_OFFSET = SF_OFFSET + SF_SLOTS * SF_BYTES;
   // plain: 32 rows x 64 bytes per draining warp; JOIN: the parts of BQ / split columns from each CTA
   static constexpr int OUT_BYTES = JOIN ? (BQ * SG_PITCH * 4 + 15) / 16 * 16 : SG_EPI_WARPS * 2048;
-  static constexpr int BAR_OFFSET = OUT_OFFSET + OUT_BYTES;
+  static constexpr int BIAS_OFFSET = OUT_OFFSET + OUT_BYTES;       // plain: the bias of a draining warp's columns
+  static constexpr int BIAS_BYTES = JOIN ? 0 : SG_EPI_WARPS * (BQ / 2) * 4;
+  static constexpr int BAR_OFFSET = BIAS_OFFSET + BIAS_BYTES;
   static constexpr int BARS = 2 * STAGES + 2 * SF_SLOTS + 2 * ACCS;
   static constexpr int TOTAL = BAR_OFFSET + 256 + 1024;
   static_assert(TOTAL <= 227 * 1024, "shared memory of one CTA");
@@ -459,8 +461,24 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constan
       int tp, tq;
       sg_tile(t, a.tiles_p, a.tiles_q, tp, tq);
       float acc[COLS];
+      if (!JOIN && a.bias != nullptr) {          // the sum starts from the bias (through shared memory: a lane has all columns)
+        float* mine = reinterpret_cast<float*>(smem + S::BIAS_OFFSET) + (warp - 4) * COLS;
+        __syncwarp();
 #pragma unroll
-      for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
+        for (int c = 0; c < COLS; c += 32) {
+          const int n = tq * BQ + c_first + c + lane;
+          mine[c + lane] = n < a.q.rows ? load_typed(a.bias, a.bias_type, n) : 0.f;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < COLS; c += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(mine + c);
+          acc[c] = v.x; acc[c + 1] = v.y; acc[c + 2] = v.z; acc[c + 3] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
+      }
       for (int c0 = kb0; c0 < kb1; c0 += a.chunk, ++it) {
         const int as = it % S::ACCS;
         const uint32_t aph = static_cast<uint32_t>(it / S::ACCS) & 1u;
@@ -542,26 +560,19 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constan
               float* dst = static_cast<float*>(a.out) + static_cast<long long>(row0) * a.ldo + col;
               if (a.vec_out && col + 16 <= width) {
                 const int piece = lane & 3;
-                float b[4] = {0.f, 0.f, 0.f, 0.f};
-                if (a.bias != nullptr) {
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) b[e] = load_typed(a.bias, a.bias_type, col + piece * 4 + e);
-                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   const int r = i * 8 + (lane >> 2);
-                  float4 o = *reinterpret_cast<const float4*>(stage + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
-                  o.x += b[0]; o.y += b[1]; o.z += b[2]; o.w += b[3];
+                  const float4 o = *reinterpret_cast<const float4*>(stage + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
                   if (r < rows) *reinterpret_cast<float4*>(dst + static_cast<long long>(r) * a.ldo + piece * 4) = o;
                 }
               } else {
                 const int e = lane & 15;
                 const bool in = col + e < width;
-                const float b = (a.bias != nullptr && in) ? load_typed(a.bias, a.bias_type, col + e) : 0.f;
 #pragma unroll 4
                 for (int r = lane >> 4; r < 32; r += 2) {
                   const float v = *reinterpret_cast<const float*>(stage + r * 64 + (((e >> 2) ^ ((r >> 1) & 3)) << 4) + (e & 3) * 4);
-                  if (in && r < rows) dst[static_cast<long long>(r) * a.ldo + e] = v + b;
+                  if (in && r < rows) dst[static_cast<long long>(r) * a.ldo + e] = v;
                 }
               }
               __syncwarp();
@@ -572,11 +583,6 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constan
           for (int c = 0; c < COLS; c += 32) {
             const int col = col0 + c;
             if (col < width && rows > 0) {
-              if (a.bias != nullptr) {          // before the rounding: every lane needs all 32 values
-                const float mine = col + lane < width ? load_typed(a.bias, a.bias_type, col + lane) : 0.f;
-#pragma unroll
-                for (int e = 0; e < 32; ++e) acc[c + e] += __shfl_sync(0xffffffffu, mine, e);
-              }
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 uint4 o;
