@@ -734,9 +734,9 @@ extern "C" int jb_scaled_gemm(const JbScaledOperand* a, const JbScaledOperand* b
   g.out = out; g.ldo = ldo; g.out_type = out_type; g.bias = bias; g.bias_type = bias_type;
   g.kblocks = static_cast<int>((K + 127) / 128);
   // The tensor cores add into TMEM by truncation, so the error of a sum grows with its length (8192 terms of random sign:
-  // 5e-7 of the result).  fp32 results are drained and added up in registers every 2048 terms; a rounding to 16 bits hides
-  // the rest of them.
-  g.chunk = out_type == JB_T_F32 ? 16 : g.kblocks;
+  // 5e-7 of the result; of one sign, up to 2^-23 for every 32 terms).  fp32 results are drained and added up in registers
+  // every 2048 terms, 16-bit ones every 16384 (2^-14 at most, an eighth of a half step of fp16).
+  g.chunk = out_type == JB_T_F32 ? 16 : 128;
   const int size = out_type == JB_T_F32 ? 4 : 2;
   g.vec_out = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (ldo * size) % 16 == 0;
   const int M = a->rows, N = b->rows;
