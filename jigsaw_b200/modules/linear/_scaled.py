@@ -17,6 +17,7 @@ from dataclasses import dataclass
 from typing import Any
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ..._core.autocast import autocast_dtype
@@ -277,7 +278,7 @@ def _check_linear(name: str, x: torch.Tensor, weight: "torch.Tensor | BlockScale
     if x.device != wc.device:
         raise ValueError(f"{name}: input on {x.device}, weight on {wc.device}")
     _check_bias(bias, N, x.device)
-    if prepared and torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+    if prepared and _traced(x, bias):
         raise ValueError(f"{name}: a prepared weight (BlockScaled) serves inference only; call it under torch.no_grad()")
     return K, N, prepared
 
@@ -285,6 +286,13 @@ def _check_linear(name: str, x: torch.Tensor, weight: "torch.Tensor | BlockScale
 def _grads(*tensors: torch.Tensor | None) -> tuple[bool, ...]:
     on = torch.is_grad_enabled()
     return tuple(on and t is not None and t.requires_grad for t in tensors)
+
+
+def _traced(*tensors: torch.Tensor | None) -> bool:
+    """A derivative is asked for: a gradient, or a tangent of forward mode."""
+    if any(_grads(*tensors)):
+        return True
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def scaled_linear(x: torch.Tensor, weight: "torch.Tensor | BlockScaled", bias: torch.Tensor | None = None) -> torch.Tensor:

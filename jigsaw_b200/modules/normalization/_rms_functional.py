@@ -34,6 +34,7 @@ from ..linear._scaled import (
     _product,
     _quantize_2d,
     _refuse_vmap,
+    _traced,
     quantize_blockwise,
 )
 
@@ -130,14 +131,14 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None = None, eps: 
     """Root-mean-square norm with the output in 8 bits (blocks of 128 features, quantised from the unrounded fp32 value):
     a :class:`BlockScaled`, or ``(BlockScaled, x + residual)`` with a residual.  For inference: not differentiable
     (:func:`rms_norm_linear` is), so tensors that want gradients are refused."""
-    if x.is_cuda and not any(_grads(x, weight, residual)):
+    if x.is_cuda and not _traced(x, weight, residual):
         out = scaled_fused.rms_norm_quantize(x, weight, eps, residual, False)
         if out is not None:
             q = _made(out[0], out[1], ROW)
             return q if residual is None else (q, out[2])
     _check("rms_norm_quantize", x, weight, residual, eps)
     _refuse_vmap("rms_norm_quantize", x, weight, residual)
-    if any(_grads(x, weight, residual)):
+    if _traced(x, weight, residual):
         raise ValueError("rms_norm_quantize has no gradient; use rms_norm_linear, or call it under torch.no_grad()")
     if residual is not None and residual.dtype != x.dtype:
         x, residual = _same_type(x, residual)
@@ -205,7 +206,7 @@ def rms_norm_linear(x: torch.Tensor, norm_weight: torch.Tensor | None, weight: "
     _refuse_vmap("rms_norm_linear", norm_weight, residual)
     if (norm_weight is not None and norm_weight.dtype not in _HALF) or (residual is not None and residual.dtype not in _HALF):
         raise TypeError("rms_norm_linear takes fp32, bf16 or fp16 tensors")
-    if prepared and any(_grads(norm_weight, residual)):
+    if prepared and _traced(norm_weight, residual):
         raise ValueError("rms_norm_linear: a prepared weight (BlockScaled) serves inference only; call it under torch.no_grad()")
     if residual is not None and residual.dtype != x.dtype:
         x, residual = _same_type(x, residual)

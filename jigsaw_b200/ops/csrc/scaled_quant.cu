@@ -991,7 +991,6 @@ static int launch_quant(const QuantArgs& a, bool tiles, int sm_count, cudaStream
 #undef JB_TILE
   } else {
     const bool vec = a.cols % 8 == 0 && (a.ldx * size) % 16 == 0 && aligned16(a.x);
-    if ((kblocks + 7) / 8 > 65535) return -1;
     const dim3 grid((a.rows + 31) / 32, (kblocks + 7) / 8);
     if (vec) launch_chained(quant_rows_kernel<T, true>, dim3(grid), dim3(256), st, 0, a);
     else launch_chained(quant_rows_kernel<T, false>, dim3(grid), dim3(256), st, 0, a);
@@ -1018,8 +1017,9 @@ extern "C" int jb_quantize(const JbQuant* q, int sm_count, void* stream) {
   a.rstd = static_cast<const float*>(q->rstd); a.gain = q->gain; a.gain_type = q->gain_type;
   a.colsum = static_cast<float*>(q->colsum); a.square = q->square;
   // rows alone: a warp per 32 rows of one block column is quick for few rows, tiles for many (8192 x 11008 bf16: 94 us
-  // against 56)
-  const bool tiles = q->square || q->codes_t != nullptr || q->rstd != nullptr || q->colsum != nullptr || q->rows >= 128;
+  // against 56); nor do 8 x 65535 block columns fit the grid of the first
+  const bool tiles = q->square || q->codes_t != nullptr || q->rstd != nullptr || q->colsum != nullptr || q->rows >= 128 ||
+                     q->cols > 65535 * 1024;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (q->type == 0) return launch_quant<float>(a, tiles, sm_count, st);
   if (q->type == 1) return launch_quant<__nv_bfloat16>(a, tiles, sm_count, st);

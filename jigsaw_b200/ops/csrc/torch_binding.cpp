@@ -519,13 +519,14 @@ struct RmsNormLinear : public Function<RmsNormLinear> {
 
 // ------------------------------------------------------------------------------------------------ Python
 // Every entry point answers None to a call that is not an ordinary one for the kernels: other types, devices or shapes that
-// do not fit, empty tensors, tensors wrapped by a transform.  The caller then takes its general path, which raises the
+// do not fit, empty tensors, tensors wrapped by a transform or whose memory does not hold their values as they are.  The caller then takes its general path, which raises the
 // error or computes the call in torch operations.
 py::object give(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
 
 bool wrapped(const Tensor& t) {
   const c10::DispatchKeySet k = t.unsafeGetTensorImpl()->key_set();
-  return k.has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Python}));
+  return k.has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Python,
+                                        c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor}));
 }
 bool float_type(const Tensor& t) {
   const at::ScalarType s = t.scalar_type();
@@ -550,6 +551,9 @@ bool norm_args(const Tensor& x, const Optional& gain, const Optional& residual, 
 }
 bool wants(const Tensor& t) { return t.requires_grad(); }
 bool wants(const Optional& t) { return t.has_value() && t->requires_grad(); }
+// A derivative is asked for, by reverse or by forward mode.
+bool traced(const Tensor& t) { return (at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined(); }
+bool traced(const Optional& t) { return t.has_value() && traced(*t); }
 
 // Type of a layer's output: that of autocast where it is on.
 int autocast_type(const Tensor& x) {
@@ -631,7 +635,7 @@ py::object py_rms_quantize(const Tensor& x, const Optional& gain, double eps, co
 // Inference forms with a prepared weight: quantisation (with or without the norm) and product, two launches.
 py::object py_linear_prepared(const Tensor& x, const Tensor& w_codes, const Tensor& w_scales, bool w_square, const Optional& bias) {
   if (!float_type(x) || x.dim() < 1 || !ordinary(x, x) || !matrix_codes(w_codes, w_scales, w_square, x) || w_codes.dim() != 2 ||
-      w_codes.size(1) != x.size(-1) || !vector_of(bias, w_codes.size(0), x) || (at::GradMode::is_enabled() && (wants(x) || wants(bias))))
+      w_codes.size(1) != x.size(-1) || !vector_of(bias, w_codes.size(0), x) || traced(x) || traced(bias))
     return py::none();
   const c10::cuda::CUDAGuard guard(x.device());
   const Quantized q = quantize(x, false, true, false, Tensor(), Tensor(), -1);
@@ -642,7 +646,7 @@ py::object py_norm_linear_prepared(const Tensor& x, const Optional& gain, double
                                    const Tensor& w_scales, bool w_square, const Optional& bias) {
   if (!norm_args(x, gain, residual, eps) || !matrix_codes(w_codes, w_scales, w_square, x) || w_codes.dim() != 2 ||
       w_codes.size(1) != x.size(-1) || !vector_of(bias, w_codes.size(0), x) ||
-      (at::GradMode::is_enabled() && (wants(x) || wants(gain) || wants(residual) || wants(bias))))
+      traced(x) || traced(gain) || traced(residual) || traced(bias))
     return py::none();
   const c10::cuda::CUDAGuard guard(x.device());
   const Normed n = rms_forward(x, opt(gain), eps, opt(residual), -1, true, false);

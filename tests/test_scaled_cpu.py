@@ -442,3 +442,24 @@ def test_names():
     for name in scaled.__all__:
         assert hasattr(scaled, name) and getattr(scaled, name).__module__ == "jigsaw_b200.modules.scaled"
     assert M.DistributedRMSNorm is scaled.DistributedRMSNorm and F.scaled_linear is scaled.scaled_linear
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be lost without a word: the forms that have no derivative refuse it like a gradient, the others have no
+    forward mode."""
+    import torch.autograd.forward_ad as fw
+
+    w = torch.ones(4, 6)
+    prepared = F.quantize_blockwise(w, SQUARE)
+    with fw.dual_level():
+        x = fw.make_dual(torch.ones(2, 6), torch.ones(2, 6))
+        gain = fw.make_dual(torch.ones(6), torch.ones(6))
+        plain = torch.ones(2, 6)
+        for call in (lambda: F.scaled_linear(x, prepared), lambda: F.rms_norm_linear(x, None, prepared),
+                     lambda: F.rms_norm_linear(plain, gain, prepared), lambda: F.rms_norm_linear(plain, None, prepared, residual=x),
+                     lambda: F.rms_norm_quantize(x), lambda: F.rms_norm_quantize(plain, gain)):
+            with pytest.raises(ValueError):
+                call()
+        for call in (lambda: F.scaled_linear(x, w), lambda: F.rms_norm_linear(x, None, w)):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()

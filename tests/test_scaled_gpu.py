@@ -210,6 +210,22 @@ def test_rows_past_32_bit_offsets():
     assert torch.equal(out[-256:], tail)
 
 
+@pytest.mark.parametrize("M, N", [(5, 300), (130, 140), (1100, 9700)])
+def test_scaled_matmul_long_rows_of_one_sign(M, N):
+    """Additions into TMEM truncate, each by up to 2^-23 of the sum so far and all in one direction: at most 512 of them (16384
+    terms, 32 at a time) before the parts are added with rounding, at most 8 parts here, so 2^-14 + 8 * 2^-24 of the result, and
+    one rounding of the result.  Summed in one go the 4096 additions could lose 2^-11, a whole half step of fp16."""
+    F = _F()
+    K = 131072 if M < 1000 else 32768
+    g = torch.Generator(device="cuda").manual_seed(0)
+    a = F.quantize_blockwise(torch.rand(M, K, generator=g, device="cuda") * 2.0**-8 + 2.0**-8)
+    b = F.quantize_blockwise(torch.rand(N, K, generator=g, device="cuda") + 1.0, SQUARE)
+    want = torch.cat([a.dequantize(torch.float64) @ part.t() for part in b.dequantize(torch.float64).split(2048)], dim=1)
+    for out in (torch.float16, torch.bfloat16):
+        y = F.scaled_matmul(a, b, out_dtype=out)
+        O.assert_within(y, want, (2.0**-14 + 2.0**-21 + O.half_step(out) * (1 + 2.0**-13)) * want, str(out))
+
+
 # ----------------------------------------------------------------------------- linear layer
 @pytest.mark.parametrize("dtype, wdtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.bfloat16, torch.bfloat16),
                                            (torch.float16, torch.float16)])
@@ -497,3 +513,59 @@ def test_layers_and_model():
     ref = torch.nn.RMSNorm(256, device="cuda")
     want = torch.nn.functional.rms_norm(x.float(), (256,), ref.weight, torch.finfo(torch.bfloat16).eps)
     torch.testing.assert_close(y, want, rtol=1e-5, atol=1e-5)
+
+
+def test_calls_inside_other_machinery():
+    """Inference mode, recomputation, batched gradients, forward mode, lazily negated inputs."""
+    import torch.autograd.forward_ad as fw
+    from torch.utils.checkpoint import checkpoint
+
+    F = _F()
+    x, w, n = _tensor(40, 256, dtype=torch.bfloat16), _tensor(64, 256, seed=1), _tensor(1, 256, seed=2)[0]
+    prepared = F.quantize_blockwise(w, SQUARE)
+    with torch.inference_mode():
+        assert torch.equal(F.scaled_linear(x, w), F.scaled_linear(x, prepared))
+        assert torch.equal(F.rms_norm_linear(x, n, w, residual=x)[0], F.rms_norm_linear(x, n, prepared, residual=x)[0])
+        assert F.distributed_rms_norm(x, n).is_inference()
+    grads = []
+    for again in (False, True):
+        leaves = [t.clone().requires_grad_() for t in (x, n, w)]
+        f = lambda x, n, w: F.rms_norm_linear(x, n, w, residual=x)  # noqa: E731
+        y, t = checkpoint(f, *leaves, use_reentrant=False) if again else f(*leaves)
+        (y.float().sum() + t.float().sum()).backward()
+        grads.append([v.grad for v in leaves])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    for f in (lambda x: F.scaled_linear(x, w), lambda x: F.distributed_rms_norm(x, n), lambda x: F.rms_norm_linear(x, n, w)):
+        leaf = x.float().requires_grad_()
+        y = f(leaf)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, leaf, torch.ones(3, *y.shape, device="cuda"), is_grads_batched=True)
+    with fw.dual_level():
+        dual = fw.make_dual(x.float(), torch.ones(40, 256, device="cuda"))
+        for f in (lambda: F.scaled_linear(dual, prepared), lambda: F.rms_norm_linear(dual, n, prepared), lambda: F.rms_norm_quantize(dual)):
+            with pytest.raises(ValueError):
+                f()
+        for f in (lambda: F.scaled_linear(dual, w), lambda: F.rms_norm_linear(dual, n, w), lambda: F.distributed_rms_norm(dual, n)):
+            with pytest.raises(RuntimeError):
+                f()
+    z = torch.complex(_tensor(40, 1), _tensor(40, 1, seed=4)).conj().imag
+    assert z.is_neg()
+    with pytest.raises(Exception, match="outside the coverage"):
+        F.quantize_blockwise(z)
+    from jigsaw_b200.ops import _lib
+
+    with _lib.strict_fused(False):
+        _same(F.quantize_blockwise(z), z.resolve_neg(), False, "negated")
+
+
+def test_quantize_few_very_long_rows():
+    """More block columns than the grid of the kernel for few rows holds."""
+    F = _F()
+    C = 65535 * 1024 + 300
+    x = torch.zeros(2, C, dtype=torch.bfloat16, device="cuda")
+    x[:, -400:] = _tensor(2, 400, dtype=torch.bfloat16)
+    q = F.quantize_blockwise(x)
+    at = (C - 400) // 128 * 128
+    tail = F.BlockScaled(q.codes[:, at:], q.scales[:, at // 128:], ROW)
+    _same(tail, x[:, at:], False, "tail")
+    assert not q.codes[:, :at].view(torch.uint8).any() and bool((q.scales[:, : at // 128].view(torch.uint8) == 127).all())
