@@ -124,8 +124,8 @@ def build_binding(force: bool = False) -> Path:
 
 
 def load_binding() -> Any:
-    """The extension module, built first if its source is newer."""
-    path = str(build_binding())
+    """The extension module (``JIGSAW_B200_BINDING``, or the in-tree one, built first if its source is newer)."""
+    path = os.environ.get("JIGSAW_B200_BINDING") or str(build_binding())
     loader = importlib.machinery.ExtensionFileLoader("_jb_torch", path)
     spec = importlib.util.spec_from_file_location("_jb_torch", path, loader=loader)
     module = importlib.util.module_from_spec(spec)

@@ -95,6 +95,9 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t local_saddr, uint32_t 
 __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
+__device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
 
 // ---------------------------------------------------------------- arguments
 enum : int { JB_T_F32 = 0, JB_T_BF16 = 1, JB_T_F16 = 2 };
@@ -138,7 +141,7 @@ struct ScaledGemmArgs {
 constexpr int SG_BP = 128;                   // rows of the operand along the lanes, per CTA
 constexpr int SG_EPI_WARPS = 8;
 constexpr int SG_THREADS = 32 * (4 + SG_EPI_WARPS);
-constexpr int SG_PITCH = SG_BP + 1;          // floats between columns of a part in shared memory
+constexpr int SG_PITCH = SG_BP + 1;          // floats between columns of a part in shared memory (SWAP)
 
 // BQ: columns of a tile.
 template <int BQ, bool PAIR, bool JOIN>
@@ -157,8 +160,9 @@ struct SgSmem {
   static constexpr int ACCS = BQ >= 256 || DUAL ? 1 : 2;           // tiles in TMEM
   static constexpr int SF_OFFSET = STAGES * KPS * TILE_BYTES;
   static constexpr int OUT_OFFSET = SF_OFFSET + SF_SLOTS * SF_BYTES;
-  // plain: 32 rows x 64 bytes per draining warp; JOIN: the parts of BQ / split columns from each CTA
-  static constexpr int OUT_BYTES = JOIN ? (BQ * SG_PITCH * 4 + 15) / 16 * 16 : SG_EPI_WARPS * 2048;
+  // plain: 32 rows x 64 bytes per draining warp; JOIN: the parts of BQ / split columns from each CTA, by columns (SWAP), or by
+  // rows with four floats between them (split up to 4)
+  static constexpr int OUT_BYTES = !JOIN ? SG_EPI_WARPS * 2048 : BQ <= 64 ? (BQ * SG_PITCH * 4 + 15) / 16 * 16 : SG_BP * (BQ + 16) * 4;
   static constexpr int BIAS_OFFSET = OUT_OFFSET + OUT_BYTES;       // plain: the bias of a draining warp's columns
   static constexpr int BIAS_BYTES = JOIN ? 0 : SG_EPI_WARPS * (BQ / 2) * 4;
   static constexpr int BAR_OFFSET = BIAS_OFFSET + BIAS_BYTES;
@@ -517,8 +521,8 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constan
         }
       }
       if constexpr (JOIN) {
-        // Column c of the tile is finished by CTA c / slots (SWAP, where few columns may be in use: c % split), at place
-        // c % slots (c / split) of what every CTA sends it.
+        // Column c of the tile is finished by CTA c / slots, in the row's place c % slots of what every CTA sends it (SWAP, where
+        // few columns may be in use: by CTA c % split, at place c / split).
         if (SWAP && split == 1) {                        // rows of the output are columns here: lanes along n
           const int n = tp * SG_BP + quad * 32 + lane;
           if (drains && n < a.p.rows) {
@@ -532,14 +536,23 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constan
           continue;
         }
         cluster_wait();                                  // all CTAs of the cluster have started
-        const uint32_t out = smem_u32(smem) + S::OUT_OFFSET + (quad * 32 + lane) * 4;
-        if (drains) {
-          const uint32_t slots = BQ / split;
+        const uint32_t slots = BQ / split;
+        if constexpr (SWAP) {
+          const uint32_t out = smem_u32(smem) + S::OUT_OFFSET + (quad * 32 + lane) * 4;
+          if (drains) {
 #pragma unroll
-          for (int c = 0; c < COLS; ++c) {
+            for (int c = 0; c < COLS; ++c) {
+              const uint32_t col = c_first + c;
+              st_cluster_f32(cluster_addr(out + (rank * slots + col / split) * (SG_PITCH * 4), col % split), acc[c]);
+            }
+          }
+        } else {
+          const uint32_t out = smem_u32(smem) + S::OUT_OFFSET + (rank * SG_BP + quad * 32 + lane) * (slots + 4) * 4;
+          const uint32_t shift = split == 4 ? 5 : 6;     // slots = 32 or 64
+#pragma unroll
+          for (int c = 0; c < COLS; c += 4) {
             const uint32_t col = c_first + c;
-            const uint32_t owner = SWAP ? col % split : col / slots, place = SWAP ? col / split : col % slots;
-            st_cluster_f32(cluster_addr(out + (rank * slots + place) * (SG_PITCH * 4), owner), acc[c]);
+            st_cluster_f32x4(cluster_addr(out + (col & (slots - 1)) * 4, col >> shift), acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
           }
         }
       } else {
@@ -641,17 +654,32 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constan
           store_typed(a.out, a.out_type, static_cast<long long>(m) * a.ldo + n, v + b);
         }
       }
-    } else {                        // lanes along the columns of the tile
-      for (int i = warp; i < SG_BP; i += SG_THREADS / 32) {
+    } else {                        // a lane takes four columns of a row
+      const int per_row = slots / 4;
+      for (int i = threadIdx.x / per_row; i < SG_BP; i += SG_THREADS / per_row) {
         const int m = tp * SG_BP + i;
         if (m >= a.p.rows) break;
-        for (int k = lane; k < slots; k += 32) {
-          const int n = tq * BQ + static_cast<int>(rank) * slots + k;
-          if (n >= a.q.rows) break;
-          float v = a.bias != nullptr ? load_typed(a.bias, a.bias_type, n) : 0.f;
-          float sum = 0.f;
-          for (int r = 0; r < static_cast<int>(split); ++r) sum += parts[(r * slots + k) * SG_PITCH + i];
-          store_typed(a.out, a.out_type, static_cast<long long>(m) * a.ldo + n, sum + v);
+        const int k = threadIdx.x % per_row * 4, n = tq * BQ + static_cast<int>(rank) * slots + k;
+        float e[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (r >= static_cast<int>(split)) break;
+          const float4 x = *reinterpret_cast<const float4*>(parts + (r * SG_BP + i) * (slots + 4) + k);
+          e[0] += x.x; e[1] += x.y; e[2] += x.z; e[3] += x.w;
+        }
+        if (a.bias != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < a.q.rows) e[j] += load_typed(a.bias, a.bias_type, n + j);
+        }
+        const long long at = static_cast<long long>(m) * a.ldo + n;
+        if (a.vec_out && n + 4 <= a.q.rows) {
+          if (a.out_type == JB_T_F32) *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(e[0], e[1], e[2], e[3]);
+          else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = make_uint2(pack_half16(e[0], e[1], a.out_type), pack_half16(e[2], e[3], a.out_type));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < a.q.rows) store_typed(a.out, a.out_type, at + j, e[j]);
         }
       }
     }
@@ -765,19 +793,20 @@ extern "C" int jb_scaled_gemm(const JbScaledOperand* a, const JbScaledOperand* b
   g.p = oa; g.q = ob;
   // Tile width.  One k-block costs a CTA about 720 cycles at 128 x 256 and 600 at 128 x 128 (shared memory, which the loads
   // fill and the products read, is the bound of both), so the wide tile wins unless it leaves a wave of SMs idle:
-  // 4096 x 1024 x 4096 takes 18 us wide and 27 us narrow, 512 x 4096 x 4096 17 us and 15.5 us.
+  // 4096 x 1024 x 4096 takes 16.9 us wide and 22.7 us narrow, 512 x 4096 x 4096 16 us and 13.5 us.
   const long long tiles256 = static_cast<long long>((M + 127) / 128) * ((N + 255) / 256);
   const long long tiles128 = static_cast<long long>((M + 127) / 128) * ((N + 127) / 128);
   const long long waves256 = (tiles256 + sm_count - 1) / sm_count, waves128 = (tiles128 + sm_count - 1) / sm_count;
   if (waves256 * 720 <= waves128 * 600) {
     // Pairs load a third less and run longer at higher clocks under the power limit (8192^3: 369 us against 430), but their
-    // hand-overs cost short products a microsecond (4096 x 4096 x 1024: 22.2 us against 21.3).
+    // hand-overs cost short products two microseconds (4096 x 4096 x 1024: 23.6 us against 21.0).
     if (g.kblocks >= 16 && tiles256 >= 2LL * sm_count) { JB_SG(256, true); }
     JB_SG(256, false);
   }
-  // A tile shared by a cluster costs about 7 us for the meeting of its parts, a k-block 0.31 us: 256 x 1024 x 8192 takes
-  // 24.8 us whole and 16.7 us in four parts, 1024 x 1024 x 4096 15.0 us whole and 19.2 us in two.
-  const int split = tiles128 * 4 <= sm_count && g.kblocks >= 32 ? 4 : tiles128 * 2 <= sm_count && g.kblocks >= 48 ? 2 : 1;
+  // A tile shared by a cluster costs 4 us (two CTAs) to 5 us (four) for the meeting of its parts, a k-block 0.26 us:
+  // 256 x 1024 x 8192 takes 20.9 us whole and 13.2 us in four parts (K = 4096: 12.6 and 11.2), 1024 x 1024 x 8192 21.2 us whole
+  // and 17.5 us in two (K = 4096: 12.9 and 13.3).
+  const int split = tiles128 * 4 <= sm_count && g.kblocks >= 32 ? 4 : tiles128 * 2 <= sm_count && g.kblocks >= 40 ? 2 : 1;
   if (split > 1) return launch_scaled_gemm<128, false, false, true>(a->codes, a->pitch, b->codes, b->pitch, K, g, split, sm_count, status, st);
   JB_SG(128, false);
 #undef JB_SG

@@ -7,7 +7,7 @@
 // smallest code is 2^-9 s).  Infinities and NaN become NaN codes and do not count towards A.
 //
 // All kernels here are bound by memory: each input byte is read once and each output byte written once.
-#include <cuda_fp8.h>
+#include <type_traits>
 
 #include "ptx.cuh"
 #include "scaled_abi.h"
@@ -38,15 +38,28 @@ __device__ __forceinline__ float code_input(float v, float inv) {
   if constexpr (CHECKED) return magnitude(v) < INF_BITS ? q : __uint_as_float(0x7fffffffu);
   return q;
 }
+// Four codes in one word, a in the lowest byte; magnitudes above 448 give 448, NaN the NaN code.
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
+  uint32_t w;
+  asm("{\n\t.reg .b16 lo, hi;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+      "mov.b32 %0, {lo, hi};\n\t}" : "=r"(w) : "f"(a), "f"(b), "f"(c), "f"(d));
+  return w;
 }
 template <bool CHECKED>
 __device__ __forceinline__ uint2 codes8(const float (&v)[8], float inv) {
   return make_uint2(codes4(code_input<CHECKED>(v[0], inv), code_input<CHECKED>(v[1], inv), code_input<CHECKED>(v[2], inv), code_input<CHECKED>(v[3], inv)),
                     codes4(code_input<CHECKED>(v[4], inv), code_input<CHECKED>(v[5], inv), code_input<CHECKED>(v[6], inv), code_input<CHECKED>(v[7], inv)));
+}
+// Four rows of four bytes -> four columns.
+__device__ __forceinline__ void turn4(uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3, uint32_t& c0, uint32_t& c1, uint32_t& c2, uint32_t& c3) {
+  const uint32_t a = __byte_perm(r0, r1, 0x5140), b = __byte_perm(r2, r3, 0x5140);
+  const uint32_t c = __byte_perm(r0, r1, 0x7362), d = __byte_perm(r2, r3, 0x7362);
+  c0 = __byte_perm(a, b, 0x5410);
+  c1 = __byte_perm(a, b, 0x7632);
+  c2 = __byte_perm(c, d, 0x5410);
+  c3 = __byte_perm(c, d, 0x7632);
 }
 // max(m, |a|, |b|), NaN if one of them is.
 __device__ __forceinline__ float max_abs3(float m, float a, float b) {
@@ -335,92 +348,102 @@ __global__ void __launch_bounds__(512, 2) quant_tile_kernel(const QuantArgs a, i
       }
     };
     share(top);
-    // not a number among the values: the rest of the tile runs on finite magnitudes, and such values leave as NaN codes
-    const bool checked = __syncthreads_or(top >= INF_BITS) != 0;
-    if (checked) {
+    // The rest of the tile, once for finite values and once for tiles with infinities or NaN: those leave as NaN codes, and
+    // the magnitudes are found again among the finite ones.
+    auto finish = [&](auto checked_c) {
+      constexpr bool CHECKED = decltype(checked_c)::value;
+      if constexpr (CHECKED) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        cm[j] = 0u;
+        for (int j = 0; j < 4; ++j) {
+          cm[j] = 0u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) cm[j] = max(cm[j], finite_magnitude(v[i][j]));
-      }
-      share(max(max(cm[0], cm[1]), max(cm[2], cm[3])));
-      __syncthreads();
-    }
-    uint32_t square_byte = 0u;
-    if (a.square) {
-      uint32_t m = 0u;
-#pragma unroll
-      for (int w = 0; w < 16; ++w) m = max(m, sh.row_mag[w]);
-      square_byte = scale_byte(m);
-      if (threadIdx.x == 0) a.scales[tile_r * a.scale_row + tile_c * a.scale_k] = static_cast<uint8_t>(square_byte);
-    } else if (a.codes_t != nullptr && threadIdx.x < 128) {
-      uint32_t m = 0u;
-#pragma unroll
-      for (int w = 0; w < 16; ++w) m = max(m, sh.col_mag[w][threadIdx.x]);
-      const uint32_t byte = scale_byte(m);
-      sh.col_inv[threadIdx.x] = inverse_scale(byte);
-      const int c = tile_c * 128 + threadIdx.x;
-      if (c < a.cols) a.scales_t[c * a.scale_t_row + tile_r * a.scale_t_k] = static_cast<uint8_t>(byte);
-    }
-    if (a.colsum != nullptr && threadIdx.x >= 128 && threadIdx.x < 256 && tile_c * 128 + threadIdx.x - 128 < a.cols) {
-      float s = 0.f;
-#pragma unroll
-      for (int w = 0; w < 16; ++w) s += sh.col_sum[w][threadIdx.x - 128];
-      a.colsum[static_cast<long long>(tile_r) * a.cols + tile_c * 128 + threadIdx.x - 128] = s;
-    }
-    if (checked) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[i][j] = code_input<true>(v[i][j], 1.f);      // NaN for every value that is not finite
-    }
-    if (a.codes != nullptr) {
-      // lane i holds the scale of row i: one computation for eight rows
-      uint32_t byte = square_byte;
-      if (!a.square) {
-        uint32_t mine = 0u;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t m = magnitude(max_abs3(max_abs3(0.f, v[i][0], v[i][1]), v[i][2], v[i][3]));
-          if (checked)
-            m = max(max(finite_magnitude(v[i][0]), finite_magnitude(v[i][1])), max(finite_magnitude(v[i][2]), finite_magnitude(v[i][3])));
-          m = __reduce_max_sync(0xffffffffu, m);
-          if (lane == i) mine = m;
+          for (int i = 0; i < 8; ++i) cm[j] = max(cm[j], finite_magnitude(v[i][j]));
         }
-        byte = scale_byte(mine);
-        if (lane < live_rows) a.scales[(row0 + lane) * a.scale_row + tile_c * a.scale_k] = static_cast<uint8_t>(byte);
+        share(max(max(cm[0], cm[1]), max(cm[2], cm[3])));
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[i][j] = code_input<true>(v[i][j], 1.f);      // NaN for every value that is not finite
+        __syncthreads();
       }
-      const float row_inv = inverse_scale(byte);
+      if (a.colsum != nullptr && threadIdx.x >= 128 && threadIdx.x < 256 && tile_c * 128 + threadIdx.x - 128 < a.cols) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) s += sh.col_sum[w][threadIdx.x - 128];
+        a.colsum[static_cast<long long>(tile_r) * a.cols + tile_c * 128 + threadIdx.x - 128] = s;
+      }
       uint8_t* out = a.codes + row0 * a.pitch + col;
-      const bool in_pitch = col < a.pitch;
-      {
+      const int out_rows = a.codes != nullptr && col < a.pitch ? live_rows : 0;
+      uint2 turned[4];                 // columns 4 l .. 4 l + 3 of this warp's eight rows
+      if (a.square) {
+        uint32_t m = 0u;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) m = max(m, sh.row_mag[w]);
+        const uint32_t byte = scale_byte(m);
+        if (threadIdx.x == 0) a.scales[tile_r * a.scale_row + tile_c * a.scale_k] = static_cast<uint8_t>(byte);
+        const float inv = inverse_scale(byte);
+        uint32_t w[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float inv = __shfl_sync(0xffffffffu, row_inv, i);
-          if (in_pitch && i < live_rows) *reinterpret_cast<uint32_t*>(out) = codes4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+          w[i] = codes4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+          if (i < out_rows) *reinterpret_cast<uint32_t*>(out) = w[i];
           out += a.pitch;
         }
-      }
-    }
-    if (a.codes_t != nullptr) {
-      float inv[4];
-      if (a.square) {
-        inv[0] = inv[1] = inv[2] = inv[3] = inverse_scale(square_byte);
+        if (a.codes_t == nullptr) return;
+        // one scale for both layouts: the codes of a column are bytes of the rows' words
+        turn4(w[0], w[1], w[2], w[3], turned[0].x, turned[1].x, turned[2].x, turned[3].x);
+        turn4(w[4], w[5], w[6], w[7], turned[0].y, turned[1].y, turned[2].y, turned[3].y);
         if (a.colsum != nullptr) __syncthreads();        // the sums have been read
       } else {
+        if (a.codes_t != nullptr && threadIdx.x < 128) {
+          uint32_t m = 0u;
+#pragma unroll
+          for (int w = 0; w < 16; ++w) m = max(m, sh.col_mag[w][threadIdx.x]);
+          const uint32_t byte = scale_byte(m);
+          sh.col_inv[threadIdx.x] = inverse_scale(byte);
+          const int c = tile_c * 128 + threadIdx.x;
+          if (c < a.cols) a.scales_t[c * a.scale_t_row + tile_r * a.scale_t_k] = static_cast<uint8_t>(byte);
+        }
+        if (a.codes != nullptr) {
+          // lane i holds the scale of row i: one computation for eight rows
+          uint32_t mine = 0u;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            uint32_t m;
+            if constexpr (CHECKED)
+              m = max(max(finite_magnitude(v[i][0]), finite_magnitude(v[i][1])), max(finite_magnitude(v[i][2]), finite_magnitude(v[i][3])));
+            else
+              m = magnitude(max_abs3(max_abs3(0.f, v[i][0], v[i][1]), v[i][2], v[i][3]));
+            m = __reduce_max_sync(0xffffffffu, m);
+            if (lane == i) mine = m;
+          }
+          const uint32_t byte = scale_byte(mine);
+          if (lane < live_rows) a.scales[(row0 + lane) * a.scale_row + tile_c * a.scale_k] = static_cast<uint8_t>(byte);
+          const float row_inv = inverse_scale(byte);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float inv = __shfl_sync(0xffffffffu, row_inv, i);
+            const uint32_t w = codes4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+            if (i < out_rows) *reinterpret_cast<uint32_t*>(out) = w;
+            out += a.pitch;
+          }
+        }
+        if (a.codes_t == nullptr) return;
         __syncthreads();
         const float4 f = *reinterpret_cast<const float4*>(&sh.col_inv[lane * 4]);
-        inv[0] = f.x; inv[1] = f.y; inv[2] = f.z; inv[3] = f.w;
+        const float inv[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float c[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) c[i] = v[i][j];
+          turned[j] = codes8<false>(c, inv[j]);
+        }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint2 q;
-        q.x = codes4(v[0][j] * inv[j], v[1][j] * inv[j], v[2][j] * inv[j], v[3][j] * inv[j]);
-        q.y = codes4(v[4][j] * inv[j], v[5][j] * inv[j], v[6][j] * inv[j], v[7][j] * inv[j]);
+      for (int j = 0; j < 4; ++j)
         // piece `warp` of column 4 lane + j, at a place that differs between the sixteen lanes of a store's half warp
-        *reinterpret_cast<uint2*>(sh.turned + (lane * 4 + j) * 128 + ((warp ^ (lane & 15)) << 3)) = q;
-      }
+        *reinterpret_cast<uint2*>(sh.turned + (lane * 4 + j) * 128 + ((warp ^ (lane & 15)) << 3)) = turned[j];
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -432,7 +455,9 @@ __global__ void __launch_bounds__(512, 2) quant_tile_kernel(const QuantArgs a, i
         if (tile_c * 128 + c < a.cols && at < a.pitch_t)
           *reinterpret_cast<uint4*>(a.codes_t + (static_cast<long long>(tile_c) * 128 + c) * a.pitch_t + at) = q;
       }
-    }
+    };
+    if (__syncthreads_or(top >= INF_BITS)) finish(std::true_type{});
+    else finish(std::false_type{});
   }
 }
 
