@@ -116,6 +116,9 @@ __device__ __forceinline__ void tc_fence_after_sync() {
 // A kernel launched with programmatic stream serialisation may start while the work queued before it still runs; nothing
 // that such work writes or reads may be touched before this point.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets such a successor start once every CTA of this grid has come here (or ended); its wait is for the end of this grid all the
+// same.  A kernel that calls it has to wait itself, so that the successor cannot overtake what ran before.
+__device__ __forceinline__ void grid_dependency_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---------------------------------------------------------------- TMA (local memory only)
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* m) {

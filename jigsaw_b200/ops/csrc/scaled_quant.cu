@@ -171,6 +171,7 @@ struct QuantArgs {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
   __shared__ __align__(8) uint8_t bytes[32][8];
+  grid_dependency_launch();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, sub = lane & 15, warp = threadIdx.x >> 5;
   const int kb0 = blockIdx.y * 8;
@@ -243,6 +244,7 @@ template <typename T, int MODE, bool NORM>
 __global__ void __launch_bounds__(512, 2) quant_tile_kernel(const QuantArgs a, int tiles_r, int tiles) {
   extern __shared__ __align__(128) uint8_t smem[];
   TileShared& sh = *reinterpret_cast<TileShared*>(smem);
+  grid_dependency_launch();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int E16 = 16 / static_cast<int>(sizeof(T));          // elements of a 16-byte copy
@@ -576,6 +578,7 @@ __device__ __forceinline__ double row_sum(double v, double* shared) {
 template <typename T, int NV, bool VEC, bool WARP, bool CODES, int MOST>
 __global__ void __launch_bounds__(MOST) rms_fwd_kernel(const RmsArgs a) {
   __shared__ double shared[32];
+  if constexpr (CODES) grid_dependency_launch();
   grid_dependency_wait();
   const int G = WARP ? 32 : blockDim.x;                          // threads of a row
   const int g = WARP ? (threadIdx.x & 31) : threadIdx.x;
@@ -869,6 +872,10 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) rms_bwd_ring_kernel(co
 // ---------------------------------------------------------------- dispatch
 // Launch that may begin while earlier work of the stream still runs: every kernel here calls grid_dependency_wait() before
 // it touches memory, so only its launch and set-up overlap (about 2 us a launch in a chain of short kernels).
+// The quantising kernels let their successor, the product, start as soon as all their CTAs have: its set-up then runs under
+// them (norm and product of 7 tokens 14.2 -> 13.4 us, in a graph 13.2; a training step of 4096 x 4096 x 1024 104.7 -> 103.1).
+// The norm's backward pass does not (its successor's CTAs would share its SMs: 182 -> 185 us at 16384 x 4096), nor does the
+// product (the next product's CTAs do not fit beside its own).
 template <typename Kernel, typename Args, typename... More>
 static cudaError_t launch_chained(Kernel kernel, dim3 grid, dim3 block, cudaStream_t stream, int smem, const Args& first, More... more) {
   cudaLaunchConfig_t cfg = {};
