@@ -272,6 +272,58 @@ def main() -> None:
         f = lambda: L.jb_halo_pack(P(src), 1, *src.stride(), NB, 3, H, W, 64, 4, P(po), None, P(ar.done_counter), st())
         return timed(f, args.warmup, args.reps), NB * H * W * (12 + 32), None      # 8-byte stores land in 32-byte sectors
 
+    # ---- 8-bit path: quantisation, root-mean-square norm, scaled products (the rate of 8-bit products is twice the peak shown)
+    from jigsaw_b200.modules import scaled
+    from jigsaw_b200.ops import scaled_fused
+
+    Rq, Cq = 8192 // scale, 11008
+    xq = torch.randn(Rq, Cq, device=dev).bfloat16()
+
+    @case("quantize_rows_cols")
+    def _():
+        f = lambda: scaled_fused.quantize_both(xq, False, True, True)
+        return timed(f, args.warmup, args.reps), Rq * Cq * (2 + 1 + 1), None
+
+    @case("quantize_squares")
+    def _():
+        f = lambda: scaled_fused.quantize_both(xq, True, True, True)
+        return timed(f, args.warmup, args.reps), Rq * Cq * (2 + 1 + 1), None
+
+    xr, res = (torch.randn(16384, 4096, device=dev).bfloat16().requires_grad_() for _ in range(2))
+    wr = torch.ones(4096, device=dev, requires_grad=True)
+
+    @case("rms_norm_fwd")
+    def _():
+        with torch.no_grad():
+            f = lambda: scaled.distributed_rms_norm(xr, wr, residual=res)
+            return timed(f, args.warmup, args.reps), xr.numel() * 2 * 4, None
+
+    @case("rms_norm_bwd")
+    def _():
+        out = scaled.distributed_rms_norm(xr, wr, residual=res)
+        g = [torch.randn_like(t) for t in out]
+        f = lambda: torch.autograd.grad(out, [xr, wr, res], g, retain_graph=True)
+        return timed(f, args.warmup, args.reps), xr.numel() * 2 * 4, None
+
+    @case("rms_norm_quantize")
+    def _():
+        with torch.no_grad():
+            f = lambda: scaled.rms_norm_quantize(xr, wr, residual=res)
+            return timed(f, args.warmup, args.reps), xr.numel() * (2 * 3 + 1), None
+
+    @case("scaled_matmul_8192x8192x8192")
+    def _():
+        a = scaled.quantize_blockwise(torch.randn(8192, 8192, device=dev).bfloat16())
+        b = scaled.quantize_blockwise(torch.randn(8192, 8192, device=dev).bfloat16(), (128, 128))
+        return timed(lambda: scaled.scaled_matmul(a, b), args.warmup, args.reps), None, 2 * 8192**3
+
+    @case("scaled_matmul_one_token")
+    def _():
+        a = scaled.quantize_blockwise(torch.randn(1, 4096, device=dev).bfloat16())
+        b = [scaled.quantize_blockwise(torch.randn(16384, 4096, device=dev).bfloat16(), (128, 128)) for _ in range(4)]   # 4 x 67 MB
+        turn = iter(range(1 << 30))
+        return timed(lambda: scaled.scaled_matmul(a, b[next(turn) % 4]), args.warmup, args.reps), 16384 * 4096, None
+
     print(f"peaks of measured: {hbm:.0f} GB/s copy, {tf:.1f} TFLOP/s cuBLAS bf16")
     for name, fn in cases.items():
         if args.only and args.only != name:
