@@ -238,8 +238,8 @@ constexpr int quant_tile_smem() { return QT_SHARED + (MODE == QT_AHEAD ? 2 * 128
 // from warp reductions, by column through shared memory, or from the whole tile; the transposed codes turn in shared
 // memory, eight bytes of a column at a time.  A CTA takes tiles in steps of the grid; of 16-bit values it has the next tile
 // copied into shared memory while it works on the present one (8192 x 11008 bf16, both layouts: 134 us with loads, which
-// the warps waited for half of the time).  Two fp32 tiles ahead would leave room for one CTA an SM, which is slower than
-// loads (11001 x 4100: 48 us against 42).
+// the warps waited for half of the time).  Two fp32 tiles ahead would leave room for one CTA an SM, which was slower
+// than loads (11001 x 4100: 48 us against 42; now 39).
 template <typename T, int MODE, bool NORM>
 __global__ void __launch_bounds__(512, 2) quant_tile_kernel(const QuantArgs a, int tiles_r, int tiles) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -1049,7 +1049,7 @@ extern "C" int jb_quantize(const JbQuant* q, int sm_count, void* stream) {
   a.rstd = static_cast<const float*>(q->rstd); a.gain = q->gain; a.gain_type = q->gain_type;
   a.colsum = static_cast<float*>(q->colsum); a.square = q->square;
   // rows alone: a warp per 32 rows of one block column is quick for few rows, tiles for many (8192 x 11008 bf16: 94 us
-  // against 56); nor do 8 x 65535 block columns fit the grid of the first
+  // against 51); nor do 8 x 65535 block columns fit the grid of the first
   const bool tiles = q->square || q->codes_t != nullptr || q->rstd != nullptr || q->colsum != nullptr || q->rows >= 128 ||
                      q->cols > 65535 * 1024;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -104,7 +104,8 @@ def test_quantize_strided_and_unaligned_inputs():
 #: pairs; one value on each axis, ends inside a tile, a k-block or a scale word
 SIZES = [(1, 1, 1), (1, 4096, 1024), (3, 130, 700), (16, 20000, 272), (17, 300, 2560), (33, 64, 128), (64, 1000, 4112),
          (65, 33, 16), (128, 128, 128), (130, 140, 5), (300, 700, 5008), (129, 257, 4099), (1000, 2056, 1000), (2048, 2048, 640),
-         (2047, 4099, 1040), (4200, 2600, 2176), (8200, 2300, 2064)]
+         (2047, 4099, 1040), (4200, 2600, 2176), (8200, 2300, 2064),
+         (1000, 1021, 5136), (700, 1096, 5200)]
 
 
 @pytest.mark.parametrize("M, N, K", SIZES)
