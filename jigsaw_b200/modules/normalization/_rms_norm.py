@@ -41,7 +41,7 @@ class DistributedRMSNorm(torch.nn.Module):
         self.local_rank = local_rank                      # kept as given; the layer takes its place from the groups
         self.device = torch.device(device)
         self.row_group, self.col_group = row_group, col_group
-        self.eps = eps                                    # None: the machine epsilon of the input's type, as in torch
+        self.eps = eps                                    # None: see _eps
         self.elementwise_affine = elementwise_affine
         local = check_divisible(normalized_dim, 1 if col_group is None else col_group.size(), "normalized_dim")
         if elementwise_affine:
@@ -73,7 +73,11 @@ class DistributedRMSNorm(torch.nn.Module):
                     dist.broadcast(p.data, group_src=0, group=self.row_group)
 
     def _eps(self, x: torch.Tensor) -> float:
-        return torch.finfo(x.dtype).eps if self.eps is None else self.eps
+        """Without an eps: the machine epsilon of the type that the norm computes in, as in ``torch.nn.RMSNorm`` (2^-23 for
+        16-bit and fp32 inputs, 2^-52 for fp64)."""
+        if self.eps is not None:
+            return self.eps
+        return torch.finfo(torch.float64 if x.dtype == torch.float64 else torch.float32).eps
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> Any:
         """``y``, or ``(y, x + residual)`` with a residual."""
