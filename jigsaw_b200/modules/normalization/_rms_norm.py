@@ -72,24 +72,25 @@ class DistributedRMSNorm(torch.nn.Module):
                 for p in self.parameters():
                     dist.broadcast(p.data, group_src=0, group=self.row_group)
 
-    def _eps(self, x: torch.Tensor) -> float:
-        """Without an eps: the machine epsilon of the type that the norm computes in, as in ``torch.nn.RMSNorm`` (2^-23 for
-        16-bit and fp32 inputs, 2^-52 for fp64)."""
+    def _eps(self, x: torch.Tensor, residual: torch.Tensor | None) -> float:
+        """Without an eps: the machine epsilon of the type that the norm of the sum computes in, as in ``torch.nn.RMSNorm``
+        (2^-52 where one of the two is fp64, else 2^-23)."""
         if self.eps is not None:
             return self.eps
-        return torch.finfo(torch.float64 if x.dtype == torch.float64 else torch.float32).eps
+        wide = x.dtype == torch.float64 or (residual is not None and residual.dtype == torch.float64)
+        return torch.finfo(torch.float64 if wide else torch.float32).eps
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> Any:
         """``y``, or ``(y, x + residual)`` with a residual."""
         (w,) = parallel.sync_grad(self.weight)
-        return distributed_rms_norm(x, w, self.col_group, self._eps(x), residual)
+        return distributed_rms_norm(x, w, self.col_group, self._eps(x, residual), residual)
 
     def forward_linear(self, x: torch.Tensor, linear: torch.nn.Module, residual: torch.Tensor | None = None) -> Any:
         """``linear(self(x, residual))``, and the sum if there is a residual.  With an 8-bit ``DistributedLinear`` whose
         input features are whole on this rank, the norm's output goes into the product as 8-bit codes."""
         if getattr(getattr(linear, "config", None), "precision", None) == "fp8" and linear.col_group.size() == 1:
             g, w, b = parallel.sync_grad(self.weight, linear.weight, linear.bias)
-            return rms_norm_linear(x, g, linear._out_block_weight(w), b, self._eps(x), residual)
+            return rms_norm_linear(x, g, linear._out_block_weight(w), b, self._eps(x, residual), residual)
         out = self(x, residual)
         return linear(out) if residual is None else (linear(out[0]), out[1])
 

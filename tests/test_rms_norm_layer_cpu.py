@@ -42,3 +42,18 @@ def test_default_eps_in_front_of_a_linear_layer(dtype):
     layer, eye = DistributedRMSNorm(64, None, "cpu", None, None, dtype=dtype), torch.nn.Identity()
     want = _want(x, 2.0**-23)
     assert bool(((layer.forward_linear(x, eye).double() - want).abs() <= _bound(want, dtype)).all())
+
+
+@pytest.mark.parametrize("dtypes", [(torch.float32, torch.float64), (torch.float64, torch.float32), (torch.bfloat16, torch.float64),
+                                    (torch.bfloat16, torch.float32)])
+def test_default_eps_is_that_of_the_sum(dtypes):
+    """What is normalised is the sum in the common type of input and residual: the order of the two changes nothing, and the norm is
+    that of the sum alone."""
+    x, r = _rows(5, 64, dtype=dtypes[0], size=2e-7), _rows(5, 64, dtype=dtypes[1], size=2e-7, seed=1)
+    common = torch.promote_types(*dtypes)
+    layer = DistributedRMSNorm(64, None, "cpu", None, None, dtype=common)
+    y, t = layer(x, r)
+    assert t.dtype == y.dtype == common
+    want = _want(t, 2.0**-52 if common == torch.float64 else 2.0**-23)
+    for got in (y, layer(r, x)[0], layer(t), layer.forward_linear(x, torch.nn.Identity(), r)[0], torch.nn.functional.rms_norm(t, (64,))):
+        assert bool(((got.double() - want).abs() <= _bound(want, common)).all())
