@@ -332,6 +332,10 @@ variable_list once(variable_list grads) {
   return grads;
 }
 
+// A gradient in memory that holds its values: autograd hands over lazily negated tensors too (the imaginary part of a
+// conjugate), whose memory has the other sign.
+Tensor stored(const Tensor& g) { return g.defined() ? g.resolve_neg() : g; }
+
 void save_codes(variable_list& to, const std::optional<Codes>& c) {
   to.push_back(c ? c->codes : Tensor());
   to.push_back(c ? c->scales : Tensor());
@@ -396,7 +400,7 @@ struct ScaledLinear : public Function<ScaledLinear> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(7);
-    const Tensor g = grads[0];
+    const Tensor g = stored(grads[0]);
     if (!g.defined()) return out;
     const c10::cuda::CUDAGuard guard(g.device());
     const variable_list s = ctx->get_saved_variables();
@@ -436,10 +440,10 @@ struct RmsNorm : public Function<RmsNorm> {
     variable_list out(6);
     const variable_list s = ctx->get_saved_variables();
     const bool residual = ctx->saved_data["residual"].toBool();
-    const Tensor gsum = residual ? grads[1] : Tensor();
+    const Tensor g = stored(grads[0]), gsum = residual ? stored(grads[1]) : Tensor();
     const bool want_gain = s[1].defined() && ctx->needs_input_grad(1);
-    if (grads[0].defined()) {
-      std::tie(out[0], out[1]) = rms_backward(s[0], s[1], s[2], grads[0], gsum, want_gain);
+    if (g.defined()) {
+      std::tie(out[0], out[1]) = rms_backward(s[0], s[1], s[2], g, gsum, want_gain);
     } else {                                   // only the sum was used
       if (gsum.defined()) out[0] = gsum.to(s[0].scalar_type());
       if (want_gain) out[1] = at::zeros_like(s[1]);
@@ -478,7 +482,7 @@ struct RmsNormLinear : public Function<RmsNormLinear> {
     const std::vector<int64_t> f = ctx->saved_data["flags"].toIntVector();
     const bool need_h = f[0], need_w = f[1], residual = f[2];
     const int64_t N = f[3];
-    const Tensor g = grads[0], gsum = residual ? grads[1] : Tensor();
+    const Tensor g = stored(grads[0]), gsum = residual ? stored(grads[1]) : Tensor();
     // edges count the tensors that were given: x, [gain], w, [bias], [residual]
     const size_t w_edge = f[6] ? 2 : 1, residual_edge = w_edge + (f[5] >= 0 ? 2 : 1);
     const int bias_type = f[5] >= 0 && ctx->needs_input_grad(w_edge + 1) ? static_cast<int>(f[5]) : -1;

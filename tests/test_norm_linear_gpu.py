@@ -1,0 +1,55 @@
+"""Gradients of the norm and of the 8-bit linear layers on the kernels, in the forms in which autograd hands them over."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _F():
+    from jigsaw_b200.modules import functional as F
+
+    return F
+
+
+def _tensor(*shape, dtype=torch.float32, seed=0, spread=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(*shape, generator=g, device="cuda") * torch.exp(spread * torch.randn(*shape[:-1], 1, generator=g, device="cuda"))
+    return x.to(dtype)
+
+
+def _calls(columns):
+    """The three operators with gradients, their outputs ``[40, columns]`` (the second also gives the sum)."""
+    F = _F()
+    x, r, w, n, b = (_tensor(*s, seed=k) for k, s in enumerate(((40, 64), (40, 64), (columns, 64), (64,), (columns,))))
+    t = _tensor(40, columns, seed=7)
+    return {
+        "linear": ((x, w, b), lambda x, w, b: (F.scaled_linear(x, w, b),)),
+        "norm linear": ((x, n, w, b, r), lambda x, n, w, b, r: F.rms_norm_linear(x, n, w, b, residual=r)),
+        "norm": ((t, t + 1, w[:, 0].clone()), lambda t, r, w: F.distributed_rms_norm(t, w, eps=0.1, residual=r)),
+    }
+
+
+@pytest.mark.parametrize("columns", [1, 24])
+@pytest.mark.parametrize("name", ["linear", "norm linear", "norm"])
+def test_lazily_negated_gradients(name, columns):
+    """The gradient of an output that becomes the imaginary part of a conjugated number arrives with its sign in a flag; with
+    one column its memory is read in place."""
+    inputs, f = _calls(columns)[name]
+    leaves = [t.clone().requires_grad_() for t in inputs]
+
+    def grads(conjugate):
+        loss = 0.0
+        for k, y in enumerate(f(*leaves)):
+            z = torch.complex(torch.zeros_like(y), y)
+            z = z.conj().imag if conjugate else -z.imag
+            loss = loss + (z * _tensor(*y.shape, seed=20 + k)).sum()
+        return torch.autograd.grad(loss, leaves)
+
+    for got, want in zip(grads(True), grads(False)):
+        assert bool(want.any()) and torch.equal(got, want)
+    # a negated gradient that lies in memory like an ordinary one
+    outs = f(*leaves)
+    gs = [_tensor(*y.shape, seed=20 + k) for k, y in enumerate(outs)]
+    got = torch.autograd.grad(outs, leaves, [torch._neg_view(g) for g in gs], retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(outs, leaves, [-g for g in gs])))
