@@ -333,8 +333,17 @@ variable_list once(variable_list grads) {
 }
 
 // A gradient in memory that holds its values: autograd hands over lazily negated tensors too (the imaginary part of a
-// conjugate), whose memory has the other sign.
-Tensor stored(const Tensor& g) { return g.defined() ? g.resolve_neg() : g; }
+// conjugate), whose memory has the other sign, and zeros without memory.
+// Tensors that a transform or a subclass wraps have none at all and are refused.
+Tensor stored(const Tensor& g) {
+  if (!g.defined()) return g;
+  const c10::DispatchKeySet k = g.unsafeGetTensorImpl()->key_set();
+  TORCH_CHECK_NOT_IMPLEMENTED(g.layout() == at::kStrided && g.is_cuda() &&
+                                  !k.has_any(c10::DispatchKeySet({c10::DispatchKey::Batched, c10::DispatchKey::FuncTorchBatched,
+                                                                  c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Python})),
+                              "the 8-bit path takes output gradients that are plain strided tensors (no torch.vmap, no wrapping subclass)");
+  return g._is_zerotensor() ? at::zeros(g.sizes(), g.options()) : g.resolve_neg();
+}
 
 void save_codes(variable_list& to, const std::optional<Codes>& c) {
   to.push_back(c ? c->codes : Tensor());

@@ -53,3 +53,38 @@ def test_lazily_negated_gradients(name, columns):
     gs = [_tensor(*y.shape, seed=20 + k) for k, y in enumerate(outs)]
     got = torch.autograd.grad(outs, leaves, [torch._neg_view(g) for g in gs], retain_graph=True)
     assert all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(outs, leaves, [-g for g in gs])))
+
+
+@pytest.mark.parametrize("name", ["linear", "norm linear", "norm"])
+def test_gradients_that_are_zeros_without_memory(name):
+    inputs, f = _calls(24)[name]
+    leaves = [t.clone().requires_grad_() for t in inputs]
+    outs = f(*leaves)
+    grads = torch.autograd.grad(outs, leaves, [torch._efficientzerotensor(y.shape, dtype=y.dtype, device=y.device) for y in outs])
+    assert all(g.shape == t.shape and not g.any() for g, t in zip(grads, leaves))
+
+
+class _Wrapped(torch.Tensor):
+    """A tensor whose values are in another one, and which has no memory of its own."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device)
+
+    def __init__(self, t):
+        self.t = t
+
+    @classmethod
+    def __torch_dispatch__(cls, f, types, args=(), kwargs=None):
+        return f(*[a.t if isinstance(a, cls) else a for a in args], **(kwargs or {}))
+
+
+@pytest.mark.parametrize("name", ["linear", "norm linear", "norm"])
+def test_wrapped_gradients_are_refused(name):
+    inputs, f = _calls(24)[name]
+    leaves = [t.clone().requires_grad_() for t in inputs]
+    outs = f(*leaves)
+    with pytest.raises(NotImplementedError):
+        torch.autograd.grad(outs, leaves, [_Wrapped(torch.ones_like(y)) for y in outs], retain_graph=True)
+    with pytest.raises(NotImplementedError):
+        torch.autograd.grad(outs, leaves, [torch.ones(3, *y.shape, device="cuda") for y in outs], is_grads_batched=True)
