@@ -116,20 +116,22 @@ class ConversionPlan:
        ``convert_to_jigsaw``);
     2. already a layer of this library                              -> keep;
     3. instance of ``shard_unsafe_modules``                          -> block (conversion refuses unless ``non_safe``);
+       an ``nn.RMSNorm`` over several axes, or over features that ``col_size`` ranks cannot share, comes here too, and every
+       ``nn.RMSNorm`` where ``convert_layer_norm`` is false (for norms over an axis that is not cut: ``non_safe`` keeps them);
     4. a leaf: elementwise (``shard_safe_modules``) -> keep, otherwise -> report;
     5. a container: descend; if it owns parameters itself           -> also report.
 
     ``apply`` then builds the replacements and re-binds them on their parents, deepest paths first, so a
     replaced child never invalidates a path still to be visited."""
 
-    def __init__(self, model: nn.Module, convert_layer_norm: bool = True) -> None:
+    def __init__(self, model: nn.Module, convert_layer_norm: bool = True, col_size: int = 1) -> None:
         self.model = model
         self.steps: list[_Step] = []
         settled: list[str] = []
         for path, module in model.named_modules():
             if any(path == root or path.startswith(root + ".") for root in settled if root) or "" in settled:
                 continue
-            step = self._decide(path, module, convert_layer_norm)
+            step = self._decide(path, module, convert_layer_norm, col_size)
             if step is None:
                 continue                                     # a plain container: its children are visited next
             self.steps.append(step)
@@ -137,12 +139,14 @@ class ConversionPlan:
                 settled.append(path)
 
     @staticmethod
-    def _decide(path: str, module: nn.Module, convert_layer_norm: bool) -> _Step | None:
+    def _decide(path: str, module: nn.Module, convert_layer_norm: bool, col_size: int) -> _Step | None:
         kind = type(module)
         skip_norm = isinstance(module, nn.LayerNorm) and not convert_layer_norm
+        uncut = kind is nn.RMSNorm and (not convert_layer_norm or len(module.normalized_shape) != 1
+                                        or module.normalized_shape[0] % col_size != 0)
         if kind in container_converters:
             return _Step(path, module, "replace", maker=container_converters[kind])
-        if kind in mapped_modules and not skip_norm:
+        if kind in mapped_modules and not skip_norm and not uncut:
             return _Step(path, module, "replace", maker=mapped_modules[kind].convert_to_jigsaw)
         if skip_norm or _is_ours(module):
             return _Step(path, module, "keep")
@@ -188,7 +192,8 @@ def convert_to_jigsaw(
     slice the same global weights.  Nothing is modified if the pre-flight check fails."""
     if on_unrecognized not in ("warn", "raise", "ignore"):
         raise ValueError(f"on_unrecognized must be 'warn', 'raise' or 'ignore', got {on_unrecognized!r}")
-    plan = ConversionPlan(model, convert_layer_norm)
+    col_size = process_mesh_dict[col_kw].size() if col_kw in process_mesh_dict else 1
+    plan = ConversionPlan(model, convert_layer_norm, col_size)
     blocked = plan.findings("block")
     if blocked and not non_safe:
         raise ValueError(

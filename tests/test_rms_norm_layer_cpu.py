@@ -57,3 +57,52 @@ def test_default_eps_is_that_of_the_sum(dtypes):
     want = _want(t, 2.0**-52 if common == torch.float64 else 2.0**-23)
     for got in (y, layer(r, x)[0], layer(t), layer.forward_linear(x, torch.nn.Identity(), r)[0], torch.nn.functional.rms_norm(t, (64,))):
         assert bool(((got.double() - want).abs() <= _bound(want, common)).all())
+
+
+# ----------------------------------------------------------------------------- conversion
+class _Group:
+    def __init__(self, n):
+        self.n = n
+
+    def size(self):
+        return self.n
+
+
+@pytest.mark.parametrize("shape, col, options", [((4, 8), 1, {}), ((8,), 3, {}), ((8,), 1, {"convert_layer_norm": False}),
+                                                 ((8,), 2, {"convert_layer_norm": False})])
+def test_norms_that_the_layer_cannot_take_are_left_to_non_safe(shape, col, options):
+    """Over several axes, over features that the column ranks cannot share, or not to be converted: refused before anything is
+    changed, and kept as plain torch with ``non_safe=True``."""
+    from jigsaw_b200 import convert
+
+    mesh = {"row": _Group(1), "col": _Group(col), "model": _Group(col)}
+    inner = torch.nn.Sequential(torch.nn.RMSNorm(shape))
+    model = torch.nn.Sequential(torch.nn.GELU(), inner)
+    with pytest.raises(ValueError, match=r"1\.0: non-elementwise module RMSNorm"):
+        convert.convert_to_jigsaw(model, mesh, "cpu", **options)
+    with pytest.warns(UserWarning, match=r"1\.0: non-elementwise module RMSNorm"):
+        out = convert.convert_to_jigsaw(model, mesh, "cpu", non_safe=True, **options)
+    assert out is model and type(inner[0]) is torch.nn.RMSNorm
+
+
+def test_a_default_half_precision_norm_keeps_its_function_through_conversion():
+    from dist_utils import run_distributed
+
+    run_distributed(_worker_convert, 2)
+
+
+def _worker_convert(rank, world):
+    import jigsaw_b200 as jb
+    from dist_utils import all_ok
+
+    mesh = jb.make_process_mesh({"row": 2, "col": 1})
+    for dtype in (torch.bfloat16, torch.float16):
+        ref = torch.nn.RMSNorm(64, dtype=dtype)
+        torch.manual_seed(0)
+        torch.nn.init.uniform_(ref.weight, 0.5, 2.0)
+        x = _rows(5, 64, dtype=dtype, size=0.01)
+        want = _want(x, 2.0**-23) * ref.weight.detach().double()
+        layer = jb.convert.convert_to_jigsaw(torch.nn.Sequential(ref), mesh, "cpu")[0]
+        assert isinstance(layer, DistributedRMSNorm)
+        for m in (layer, ref, layer.convert_to_torch(mesh)):
+            assert all_ok(bool(((m(x).detach().double() - want).abs() <= 2 * _bound(want, dtype)).all()))
