@@ -17,7 +17,14 @@ import torch.distributed as dist
 from ... import parallel
 from ..._core.placement import check_divisible, gather_dim
 from ..._core.shard_repr import shard_repr
+from ..linear._linear import DistributedLinear
 from ._rms_functional import distributed_rms_norm, rms_norm_linear
+
+
+def _called_plainly(module: torch.nn.Module, kind: type) -> bool:
+    """A call of ``module`` runs ``kind.forward`` and nothing else: no hook, no forward of a subclass or of the instance."""
+    return (type(module).forward is kind.forward and "forward" not in vars(module)
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
 
 
 class DistributedRMSNorm(torch.nn.Module):
@@ -87,8 +94,12 @@ class DistributedRMSNorm(torch.nn.Module):
 
     def forward_linear(self, x: torch.Tensor, linear: torch.nn.Module, residual: torch.Tensor | None = None) -> Any:
         """``linear(self(x, residual))``, and the sum if there is a residual.  With an 8-bit ``DistributedLinear`` whose
-        input features are whole on this rank, the norm's output goes into the product as 8-bit codes."""
-        if getattr(getattr(linear, "config", None), "precision", None) == "fp8" and linear.col_group.size() == 1:
+        input features are whole on this rank, the norm's output goes into the product as 8-bit codes, unless something
+        watches or replaces a call of one of the two (hooks, an own ``forward``): then both modules are called, and the norm's
+        output is rounded to its type in between."""
+        if (_called_plainly(self, DistributedRMSNorm) and isinstance(linear, DistributedLinear) and _called_plainly(linear, DistributedLinear)
+                and linear.config.precision == "fp8" and linear.col_group.size() == 1
+                and not torch.nn.modules.module._has_any_global_hook()):
             g, w, b = parallel.sync_grad(self.weight, linear.weight, linear.bias)
             return rms_norm_linear(x, g, linear._out_block_weight(w), b, self._eps(x, residual), residual)
         out = self(x, residual)
