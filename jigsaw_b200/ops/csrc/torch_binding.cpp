@@ -205,12 +205,12 @@ Quantized quantize(const Tensor& input, bool square, bool want_rows, bool want_c
 
 // a [M, K] b [N, K]^T + bias, as a tensor of the given sizes (M N elements).
 Tensor product(const JbScaledOperand& a, const JbScaledOperand& b, int64_t K, const Tensor& bias, int out_type,
-               at::IntArrayRef sizes, const Tensor& like, const Tensor& status) {
+               at::IntArrayRef sizes, const Tensor& like) {
   Tensor out = empty(sizes, scalar_of(out_type), like);
   Tensor bias_c;
   if (bias.defined()) bias_c = bias.contiguous();
   done(api.gemm(&a, &b, K, out.data_ptr(), b.rows, out_type, bias.defined() ? bias_c.const_data_ptr() : nullptr,
-                bias.defined() ? type_of(bias_c.scalar_type()) : 0, sm_count(like), status.data_ptr<int>(), stream_of(like)),
+                bias.defined() ? type_of(bias_c.scalar_type()) : 0, sm_count(like), status_of(like).data_ptr<int>(), stream_of(like)),
        "scaled_gemm");
   return out;
 }
@@ -372,12 +372,12 @@ struct LinearGrads {
 };
 // The two gradient products of a layer whose transposed weight and column-quantised input are given (absent: not wanted).
 LinearGrads linear_backward(const Tensor& g, const std::optional<Codes>& w_t, const std::optional<Codes>& x_t, int dx_type,
-                            at::IntArrayRef dx_sizes, int dw_type, int bias_type, const Tensor& status) {
+                            at::IntArrayRef dx_sizes, int dw_type, int bias_type) {
   LinearGrads out;
   const Quantized q = quantize(g, false, w_t.has_value(), x_t.has_value(), Tensor(), Tensor(), bias_type);
   const int64_t N = g.size(-1), M = g.numel() / N;
-  if (w_t) out.dx = product(q.rows->operand(), w_t->operand(), N, Tensor(), dx_type, dx_sizes, g, status);
-  if (x_t) out.dw = product(q.cols->operand(), x_t->operand(), M, Tensor(), dw_type, {N, x_t->rows}, g, status);
+  if (w_t) out.dx = product(q.rows->operand(), w_t->operand(), N, Tensor(), dx_type, dx_sizes, g);
+  if (x_t) out.dw = product(q.cols->operand(), x_t->operand(), M, Tensor(), dw_type, {N, x_t->rows}, g);
   out.db = q.sums;
   return out;
 }
@@ -389,7 +389,7 @@ Tensor bias_sum(const Tensor& g, int type) {
 // written in the layouts that all three products want.
 struct ScaledLinear : public Function<ScaledLinear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Optional& bias, int64_t out_type, bool need_x,
-                        bool need_w, const Tensor& status) {
+                        bool need_w) {
     const Tensor b = opt(bias);
     const c10::cuda::CUDAGuard guard(x.device());
     const Quantized qx = quantize(x, false, true, need_w, Tensor(), Tensor(), -1);
@@ -397,18 +397,17 @@ struct ScaledLinear : public Function<ScaledLinear> {
     variable_list save;
     save_codes(save, qx.cols);
     save_codes(save, qw.cols);
-    save.push_back(status);
     ctx->save_for_backward(save);
     ctx->saved_data["x"] = x.sizes().vec();
     ctx->saved_data["n"] = w.size(0);
     ctx->saved_data["types"] = std::vector<int64_t>{type_of(x.scalar_type()), type_of(w.scalar_type()),
                                                     b.defined() ? type_of(b.scalar_type()) : -1};
     ctx->set_materialize_grads(false);
-    return product(qx.rows->operand(), qw.rows->operand(), x.size(-1), b, static_cast<int>(out_type), with_last(x, w.size(0)), x, status);
+    return product(qx.rows->operand(), qw.rows->operand(), x.size(-1), b, static_cast<int>(out_type), with_last(x, w.size(0)), x);
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list out(7);
+    variable_list out(6);
     const Tensor g = stored(grads[0]);
     if (!g.defined()) return out;
     const c10::cuda::CUDAGuard guard(g.device());
@@ -422,7 +421,7 @@ struct ScaledLinear : public Function<ScaledLinear> {
     if (s[2].defined() && ctx->needs_input_grad(0)) w_t = saved_codes(s[2], s[3], K, N, true);
     const int bias_type = types[2] >= 0 && ctx->needs_input_grad(2) ? static_cast<int>(types[2]) : -1;
     if (x_t || w_t) {
-      LinearGrads l = linear_backward(g, w_t, x_t, static_cast<int>(types[0]), xs, static_cast<int>(types[1]), bias_type, s[4]);
+      LinearGrads l = linear_backward(g, w_t, x_t, static_cast<int>(types[0]), xs, static_cast<int>(types[1]), bias_type);
       out[0] = l.dx;
       out[1] = l.dw;
       out[2] = l.db;
@@ -466,8 +465,7 @@ struct RmsNorm : public Function<RmsNorm> {
 // blocks of the weight gradient, and keeps the gradient of the normalised rows in fp32 between product and norm.
 struct RmsNormLinear : public Function<RmsNormLinear> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Optional& gain_in, const Tensor& w, const Optional& bias,
-                               const Optional& residual_in, double eps, int64_t out_type, bool need_h, bool need_w,
-                               const Tensor& status) {
+                               const Optional& residual_in, double eps, int64_t out_type, bool need_h, bool need_w) {
     const Tensor gain = opt(gain_in), b = opt(bias), residual = opt(residual_in);
     const c10::cuda::CUDAGuard guard(x.device());
     Normed n = rms_forward(x, gain, eps, residual, -1, true, need_h || need_w);
@@ -477,17 +475,16 @@ struct RmsNormLinear : public Function<RmsNormLinear> {
     if (need_h || need_w) {
       save = {residual.defined() ? n.sum : x, gain, n.rstd};
       save_codes(save, qw.cols);
-      save.push_back(status);
     }
     ctx->save_for_backward(save);
     ctx->saved_data["flags"] = std::vector<int64_t>{need_h, need_w, residual.defined(), w.size(0), type_of(w.scalar_type()),
                                                     b.defined() ? type_of(b.scalar_type()) : -1, gain.defined()};
-    Tensor y = product(n.codes->operand(), qw.rows->operand(), x.size(-1), b, static_cast<int>(out_type), with_last(x, w.size(0)), x, status);
+    Tensor y = product(n.codes->operand(), qw.rows->operand(), x.size(-1), b, static_cast<int>(out_type), with_last(x, w.size(0)), x);
     return residual.defined() ? variable_list{y, n.sum} : variable_list{y};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list out(10);
+    variable_list out(9);
     const std::vector<int64_t> f = ctx->saved_data["flags"].toIntVector();
     const bool need_h = f[0], need_w = f[1], residual = f[2];
     const int64_t N = f[3];
@@ -511,7 +508,7 @@ struct RmsNormLinear : public Function<RmsNormLinear> {
       if (want_h) w_t = saved_codes(s[3], s[4], K, N, true);
       if (need_w && ctx->needs_input_grad(w_edge)) h_t = quantize(t, false, false, true, rstd, gain, -1).cols;
       if (w_t || h_t) {
-        LinearGrads l = linear_backward(g, w_t, h_t, 0, t.sizes(), static_cast<int>(f[4]), bias_type, s[5]);
+        LinearGrads l = linear_backward(g, w_t, h_t, 0, t.sizes(), static_cast<int>(f[4]), bias_type);
         dh = l.dx;
         out[2] = l.dw;
         out[3] = l.db;
@@ -631,7 +628,7 @@ py::object py_scaled_matmul(const Tensor& a_codes, const Tensor& a_scales, bool 
     return py::none();
   const c10::cuda::CUDAGuard guard(a_codes.device());
   const Codes a = operand_of(a_codes, a_scales, a_square), b = operand_of(b_codes, b_scales, b_square);
-  return give(product(describe(a), describe(b), a.cols, opt(bias), out_type, with_last(a_codes, b.rows), a_codes, status_of(a_codes)));
+  return give(product(describe(a), describe(b), a.cols, opt(bias), out_type, with_last(a_codes, b.rows), a_codes));
 }
 
 py::object py_rms_quantize(const Tensor& x, const Optional& gain, double eps, const Optional& residual, bool want_rstd) {
@@ -653,7 +650,7 @@ py::object py_linear_prepared(const Tensor& x, const Tensor& w_codes, const Tens
   const c10::cuda::CUDAGuard guard(x.device());
   const Quantized q = quantize(x, false, true, false, Tensor(), Tensor(), -1);
   const Codes w = operand_of(w_codes, w_scales, w_square);
-  return give(product(q.rows->operand(), describe(w), w.cols, opt(bias), autocast_type(x), with_last(x, w.rows), x, status_of(x)));
+  return give(product(q.rows->operand(), describe(w), w.cols, opt(bias), autocast_type(x), with_last(x, w.rows), x));
 }
 py::object py_norm_linear_prepared(const Tensor& x, const Optional& gain, double eps, const Optional& residual, const Tensor& w_codes,
                                    const Tensor& w_scales, bool w_square, const Optional& bias) {
@@ -664,7 +661,7 @@ py::object py_norm_linear_prepared(const Tensor& x, const Optional& gain, double
   const c10::cuda::CUDAGuard guard(x.device());
   const Normed n = rms_forward(x, opt(gain), eps, opt(residual), -1, true, false);
   const Codes w = operand_of(w_codes, w_scales, w_square);
-  return py::make_tuple(give(product(n.codes->operand(), describe(w), w.cols, opt(bias), autocast_type(x), with_last(x, w.rows), x, status_of(x))),
+  return py::make_tuple(give(product(n.codes->operand(), describe(w), w.cols, opt(bias), autocast_type(x), with_last(x, w.rows), x)),
                         give(n.sum));
 }
 
@@ -674,7 +671,7 @@ bool weight_args(const Tensor& x, const Tensor& w, const Optional& b) {
 py::object py_scaled_linear(const Tensor& x, const Tensor& w, const Optional& b) {
   if (!float_type(x) || x.dim() < 1 || !ordinary(x, x) || !weight_args(x, w, b)) return py::none();
   const bool grad = at::GradMode::is_enabled();
-  return give(ScaledLinear::apply(x, w, b, static_cast<int64_t>(autocast_type(x)), grad && wants(x), grad && wants(w), status_of(x)));
+  return give(ScaledLinear::apply(x, w, b, static_cast<int64_t>(autocast_type(x)), grad && wants(x), grad && wants(w)));
 }
 py::tuple pair_of(const variable_list& v) { return py::make_tuple(give(v[0]), v.size() > 1 ? give(v[1]) : py::none()); }
 py::object py_rms_norm(const Tensor& x, const Optional& gain, const Optional& residual, double eps) {
@@ -688,7 +685,7 @@ py::object py_rms_norm_linear(const Tensor& x, const Optional& gain, const Tenso
   if (!norm_args(x, gain, residual, eps) || !weight_args(x, w, b)) return py::none();
   const bool grad = at::GradMode::is_enabled();
   return pair_of(RmsNormLinear::apply(x, gain, w, b, residual, eps, static_cast<int64_t>(autocast_type(x)),
-                                      grad && (wants(x) || wants(gain) || wants(residual)), grad && wants(w), status_of(x)));
+                                      grad && (wants(x) || wants(gain) || wants(residual)), grad && wants(w)));
 }
 
 void init(const py::dict& entry) {

@@ -88,3 +88,20 @@ def test_wrapped_gradients_are_refused(name):
         torch.autograd.grad(outs, leaves, [_Wrapped(torch.ones_like(y)) for y in outs], retain_graph=True)
     with pytest.raises(NotImplementedError):
         torch.autograd.grad(outs, leaves, [torch.ones(3, *y.shape, device="cuda") for y in outs], is_grads_batched=True)
+
+
+@pytest.mark.parametrize("name", ["linear", "norm linear"])
+def test_the_status_word_may_be_reset_between_forward_and_backward(name):
+    """``check_status`` clears it after an error that some other kernel recorded; the graph of a sound step is not part of that."""
+    from jigsaw_b200.ops import symm
+
+    inputs, f = _calls(24)[name]
+    leaves = [t.clone().requires_grad_() for t in inputs]
+    gs = [_tensor(*y.shape, seed=20 + k) for k, y in enumerate(f(*inputs))]
+    want = torch.autograd.grad(f(*leaves), leaves, gs)
+    outs = f(*leaves)
+    status = symm.arena(outs[0].device)
+    status.status[0] = 1
+    with pytest.raises(RuntimeError, match="kernel error 1"):
+        status.check_status()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(outs, leaves, gs), want))
