@@ -88,6 +88,18 @@ __device__ __forceinline__ uint32_t block_of_16_lanes(const float (&v)[8], uint2
   return byte;
 }
 
+// Sum and product that keep results below 2^-126 (the library is compiled with fast math, which makes them zero).
+__device__ __forceinline__ float add_full(float a, float b) {
+  float r;
+  asm("add.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float mul_full(float a, float b) {
+  float r;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -319,7 +331,7 @@ __global__ void __launch_bounds__(512, 2) quant_tile_kernel(const QuantArgs a, i
       for (int i = 0; i < 8; ++i) {
         const float r = i < live_rows ? __ldg(a.rstd + row0 + i) : 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[i][j] = v[i][j] * r * g[j];
+        for (int j = 0; j < 4; ++j) v[i][j] = mul_full(mul_full(v[i][j], r), g[j]);
       }
     }
     uint32_t cm[4];
@@ -602,7 +614,7 @@ __global__ void __launch_bounds__(MOST) rms_fwd_kernel(const RmsArgs a) {
     for (int i = 0; i < NV; ++i) {
       // the norm is of the sum as it is stored: the backward pass, which reads the stored one, differentiates this function
 #pragma unroll
-      for (int e = 0; e < 8; ++e) t[i][e] = to_f32<T>(from_f32<T>(t[i][e] + to_f32<T>(r[i][e])));
+      for (int e = 0; e < 8; ++e) t[i][e] = to_f32<T>(from_f32<T>(add_full(t[i][e], to_f32<T>(r[i][e]))));
       store8<T, VEC>(sum, column(i), step, a.cols, t[i]);
     }
   }
@@ -620,7 +632,7 @@ __global__ void __launch_bounds__(MOST) rms_fwd_kernel(const RmsArgs a) {
     float w[8];
     gain8<VEC>(a.gain, a.gain_type, c, step, a.cols, w);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) t[i][e] = t[i][e] * rstd * w[e];
+    for (int e = 0; e < 8; ++e) t[i][e] = mul_full(mul_full(t[i][e], rstd), w[e]);
     if constexpr (CODES) {
       uint2 q;
       const uint32_t byte = block_of_16_lanes(t[i], q);          // 16 lanes = 128 columns

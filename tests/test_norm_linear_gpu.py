@@ -105,3 +105,23 @@ def test_the_status_word_may_be_reset_between_forward_and_backward(name):
     with pytest.raises(RuntimeError, match="kernel error 1"):
         status.check_status()
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(outs, leaves, gs), want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("C", [64, 65, 5000])
+def test_sums_and_outputs_below_the_normal_range(C, dtype):
+    """The stored sum is the rounded sum of the two tensors at every size, and the norm is of that sum: values below 2^-126 are
+    not flushed to zero on the way in."""
+    F = _F()
+    g = torch.Generator(device="cuda").manual_seed(0)
+    step = 2.0**-149 if dtype == torch.float32 else 2.0**-133
+    x, r = (torch.randint(-(2**6), 2**6, (7, C), generator=g, device="cuda").double() * step for _ in range(2))
+    x[:, 0], r[:, 0] = 2.0**-126, -(2.0**-126) + step
+    x, r = x.to(dtype), r.to(dtype)
+    gain = torch.full((C,), 2.0**20, device="cuda")
+    want = x.double() + r.double()
+    y, t = F.distributed_rms_norm(x, gain, eps=2.0**-40, residual=r)
+    assert torch.equal(t.double(), want) and bool(want.any())
+    # r = 2^20 exactly, and two products by powers of two: one rounding to the type
+    assert torch.equal(y, (want * 2.0**40).to(dtype))
+    assert torch.equal(F.rms_norm_quantize(x, gain, 2.0**-40, r)[1].double(), want)
