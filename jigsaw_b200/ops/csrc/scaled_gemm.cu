@@ -761,9 +761,11 @@ extern "C" int jb_scaled_gemm(const JbScaledOperand* a, const JbScaledOperand* b
   const ScaledOperand oa = operand(a), ob = operand(b);
   g.out = out; g.ldo = ldo; g.out_type = out_type; g.bias = bias; g.bias_type = bias_type;
   g.kblocks = static_cast<int>((K + 127) / 128);
-  // The tensor cores add into TMEM by truncation, so the error of a sum grows with its length (8192 terms of random sign:
-  // 5e-7 of the result; of one sign, up to 2^-23 for every 32 terms).  fp32 results are drained and added up in registers
-  // every 2048 terms, 16-bit ones every 16384 (2^-14 at most, an eighth of a half step of fp16).
+  // The tensor cores add into TMEM by truncation: every addition (32 terms) loses up to 2^-23 of the sum so far, all towards
+  // zero, so the error of a sum grows with its length and is relative to the sum of its terms' magnitudes S, not to the result
+  // (8192 terms of random sign: 5e-7 of the result).  fp32 results are drained and added up in registers every 2048 terms
+  // (2^-17 S at most), 16-bit ones every 16384 (2^-14 S at most: an eighth of a half step of fp16 where all terms have one
+  // sign; where they cancel, more of the result, like any fp32 sum, which may lose K 2^-24 S).
   g.chunk = out_type == JB_T_F32 ? 16 : 128;
   const int size = out_type == JB_T_F32 ? 4 : 2;
   g.vec_out = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (ldo * size) % 16 == 0;

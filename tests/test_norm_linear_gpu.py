@@ -125,3 +125,28 @@ def test_sums_and_outputs_below_the_normal_range(C, dtype):
     # r = 2^20 exactly, and two products by powers of two: one rounding to the type
     assert torch.equal(y, (want * 2.0**40).to(dtype))
     assert torch.equal(F.rms_norm_quantize(x, gain, 2.0**-40, r)[1].double(), want)
+
+
+@pytest.mark.parametrize("out", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M, N, K", [(5, 300, 131072), (130, 140, 131072), (1100, 9700, 32768)])
+def test_scaled_matmul_long_rows_that_cancel(M, N, K, out):
+    """The loss of the truncating additions is relative to the sum of magnitudes S: 16-bit results take at most 512 of them in a
+    row (fp32: 64), each up to 2^-23 S, then K / 16384 (fp32: K / 2048) rounded additions of what was drained and at most 16 of
+    parts (two accumulators, eight CTAs), and one rounding."""
+    F = _F()
+    g = torch.Generator(device="cuda").manual_seed(0)
+    a = torch.rand(M, K, generator=g, device="cuda") + 1.0
+    sign = torch.ones(K, device="cuda")
+    sign[K // 2:] = -1.0                         # what the first half of a row adds up, the second takes away
+    a = F.quantize_blockwise(a * sign * 2.0**-8)
+    b = F.quantize_blockwise(torch.rand(N, K, generator=g, device="cuda") + 1.0, (128, 128))
+    va = a.dequantize(torch.float64)
+    parts = b.dequantize().split(1024)
+    want = torch.cat([va @ p.double().t() for p in parts], dim=1)
+    total = torch.cat([va.abs() @ p.double().abs().t() for p in parts], dim=1)
+    assert float(want.abs().median()) < 0.02 * float(total.median()), "the sums cancel"
+    chunk = 2048 if out == torch.float32 else 16384
+    bound = (chunk // 32 * 2.0**-23 + (K // chunk + 16) * 2.0**-24) * total
+    half = torch.finfo(out).eps / 2
+    y = F.scaled_matmul(a, b, out_dtype=out).double()
+    assert bool(((y - want).abs() <= bound * (1 + half) + half * want.abs() + 2.0**-25).all())
