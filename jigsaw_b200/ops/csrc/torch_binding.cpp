@@ -332,6 +332,13 @@ variable_list once(variable_list grads) {
   return grads;
 }
 
+// Its memory does not hold its values as they are, or it has none: wrapped by a transform or a subclass, lazily negated, zeros.
+bool wrapped(const Tensor& t) {
+  const c10::DispatchKeySet k = t.unsafeGetTensorImpl()->key_set();
+  return k.has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Python,
+                                        c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor}));
+}
+
 // A gradient in memory that holds its values: autograd hands over lazily negated tensors too (the imaginary part of a
 // conjugate), whose memory has the other sign, and zeros without memory.
 // Tensors that a transform or a subclass wraps have none at all and are refused.
@@ -349,16 +356,36 @@ void save_codes(variable_list& to, const std::optional<Codes>& c) {
   to.push_back(c ? c->codes : Tensor());
   to.push_back(c ? c->scales : Tensor());
 }
+bool float_type(const Tensor& t) {
+  const at::ScalarType s = t.scalar_type();
+  return s == at::kFloat || s == at::kBFloat16 || s == at::kHalf;
+}
+// What the forward pass saved, as it comes back: saved-tensor hooks may hand over another tensor in its place, at other
+// strides (then it is copied), or one that the kernels must not be given.
+Tensor restored(const Tensor& t, at::ScalarType type, at::IntArrayRef sizes, const Tensor& g) {
+  TORCH_CHECK(t.defined() && t.device() == g.device() && t.layout() == at::kStrided && !wrapped(t) && t.scalar_type() == type && t.sizes() == sizes,
+              "a tensor that the 8-bit path saved for its backward pass came back from a saved-tensor hook as another one (device, type or shape)");
+  return t.contiguous();
+}
+// The same for a tensor that the kernels take at any strides and in any of their types.
+const Tensor& restored(const Tensor& t, int64_t rows, int64_t cols, const Tensor& g) {
+  TORCH_CHECK(t.defined() && t.device() == g.device() && t.layout() == at::kStrided && !wrapped(t) && float_type(t) && t.dim() >= 1 &&
+                  t.size(-1) == cols && t.numel() == rows * cols,
+              "a tensor that the 8-bit path saved for its backward pass came back from a saved-tensor hook as another one (device, type or shape)");
+  return t;
+}
 // The transposed weight, or the activations in blocks along the tokens, as saved by the forward pass.
-Codes saved_codes(const Tensor& codes, const Tensor& scales, int64_t rows, int64_t cols, bool square) {
+Codes saved_codes(const Tensor& codes, const Tensor& scales, int64_t rows, int64_t cols, bool square, const Tensor& g) {
+  const int64_t rb = (rows + 127) / 128, cb = (cols + 127) / 128;
   Codes c;
-  c.codes = codes;
-  c.scales = scales;
+  c.codes = restored(codes, CODES, {rows, pitch_of(cols)}, g);
+  // of a square the scales are those of the matrix that was not turned
+  c.scales = square ? restored(scales, SCALES, {cb, words_of(rb)}, g) : restored(scales, SCALES, {rows, words_of(cb)}, g);
   c.rows = rows;
   c.cols = cols;
   c.square = c.turned = square;
-  c.scale_row = square ? 1 : scales.size(1);
-  c.scale_k = square ? scales.size(1) : 1;
+  c.scale_row = square ? 1 : c.scales.size(1);
+  c.scale_k = square ? c.scales.size(1) : 1;
   return c;
 }
 std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
@@ -417,8 +444,8 @@ struct ScaledLinear : public Function<ScaledLinear> {
     int64_t M = 1;
     for (size_t i = 0; i + 1 < xs.size(); ++i) M *= xs[i];
     std::optional<Codes> x_t, w_t;
-    if (s[0].defined() && ctx->needs_input_grad(1)) x_t = saved_codes(s[0], s[1], K, M, false);
-    if (s[2].defined() && ctx->needs_input_grad(0)) w_t = saved_codes(s[2], s[3], K, N, true);
+    if (s[0].defined() && ctx->needs_input_grad(1)) x_t = saved_codes(s[0], s[1], K, M, false, g);
+    if (s[2].defined() && ctx->needs_input_grad(0)) w_t = saved_codes(s[2], s[3], K, N, true, g);
     const int bias_type = types[2] >= 0 && ctx->needs_input_grad(2) ? static_cast<int>(types[2]) : -1;
     if (x_t || w_t) {
       LinearGrads l = linear_backward(g, w_t, x_t, static_cast<int>(types[0]), xs, static_cast<int>(types[1]), bias_type);
@@ -451,7 +478,9 @@ struct RmsNorm : public Function<RmsNorm> {
     const Tensor g = stored(grads[0]), gsum = residual ? stored(grads[1]) : Tensor();
     const bool want_gain = s[1].defined() && ctx->needs_input_grad(1);
     if (g.defined()) {
-      std::tie(out[0], out[1]) = rms_backward(s[0], s[1], s[2], g, gsum, want_gain);
+      const int64_t cols = g.size(-1), rows = g.numel() / cols;
+      if (s[1].defined()) restored(s[1], 1, cols, g);
+      std::tie(out[0], out[1]) = rms_backward(restored(s[0], rows, cols, g), s[1], restored(s[2], at::kFloat, {rows}, g), g, gsum, want_gain);
     } else {                                   // only the sum was used
       if (gsum.defined()) out[0] = gsum.to(s[0].scalar_type());
       if (want_gain) out[1] = at::zeros_like(s[1]);
@@ -478,7 +507,7 @@ struct RmsNormLinear : public Function<RmsNormLinear> {
     }
     ctx->save_for_backward(save);
     ctx->saved_data["flags"] = std::vector<int64_t>{need_h, need_w, residual.defined(), w.size(0), type_of(w.scalar_type()),
-                                                    b.defined() ? type_of(b.scalar_type()) : -1, gain.defined()};
+                                                    b.defined() ? type_of(b.scalar_type()) : -1, gain.defined(), x.size(-1)};
     Tensor y = product(n.codes->operand(), qw.rows->operand(), x.size(-1), b, static_cast<int>(out_type), with_last(x, w.size(0)), x);
     return residual.defined() ? variable_list{y, n.sum} : variable_list{y};
   }
@@ -497,15 +526,19 @@ struct RmsNormLinear : public Function<RmsNormLinear> {
       if (g.defined() && bias_type >= 0) out[3] = bias_sum(g, bias_type);
       return once(std::move(out));
     }
-    const Tensor &t = s[0], &gain = s[1], &rstd = s[2];
-    const c10::cuda::CUDAGuard guard(t.device());
-    const int64_t K = t.size(-1);
+    const Tensor &t = s[0], &gain = s[1];
+    const int64_t K = f[7];
     const bool want_gain = gain.defined() && ctx->needs_input_grad(1);
     const bool want_h = need_h && (want_gain || ctx->needs_input_grad(0) || (residual && ctx->needs_input_grad(residual_edge)));
-    Tensor dh;
+    Tensor dh, rstd;
     if (g.defined()) {
+      const c10::cuda::CUDAGuard guard(g.device());
+      const int64_t M = g.numel() / N;
+      restored(t, M, K, g);
+      if (gain.defined()) restored(gain, 1, K, g);
+      rstd = restored(s[2], at::kFloat, {M}, g);
       std::optional<Codes> w_t, h_t;
-      if (want_h) w_t = saved_codes(s[3], s[4], K, N, true);
+      if (want_h) w_t = saved_codes(s[3], s[4], K, N, true, g);
       if (need_w && ctx->needs_input_grad(w_edge)) h_t = quantize(t, false, false, true, rstd, gain, -1).cols;
       if (w_t || h_t) {
         LinearGrads l = linear_backward(g, w_t, h_t, 0, t.sizes(), static_cast<int>(f[4]), bias_type);
@@ -529,19 +562,10 @@ struct RmsNormLinear : public Function<RmsNormLinear> {
 
 // ------------------------------------------------------------------------------------------------ Python
 // Every entry point answers None to a call that is not an ordinary one for the kernels: other types, devices or shapes that
-// do not fit, empty tensors, tensors wrapped by a transform or whose memory does not hold their values as they are.  The caller then takes its general path, which raises the
-// error or computes the call in torch operations.
+// do not fit, empty tensors, tensors wrapped by a transform or whose memory does not hold their values as they are.  The
+// caller then takes its general path, which raises the error or computes the call in torch operations.
 py::object give(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
 
-bool wrapped(const Tensor& t) {
-  const c10::DispatchKeySet k = t.unsafeGetTensorImpl()->key_set();
-  return k.has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Python,
-                                        c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor}));
-}
-bool float_type(const Tensor& t) {
-  const at::ScalarType s = t.scalar_type();
-  return s == at::kFloat || s == at::kBFloat16 || s == at::kHalf;
-}
 bool ordinary(const Tensor& t, const Tensor& like) {
   return t.layout() == at::kStrided && t.device() == like.device() && t.is_cuda() && !wrapped(t) && t.numel() > 0;
 }

@@ -344,3 +344,39 @@ def _worker_vit(rank, world):
 
 def test_vit_with_rms_norms_and_8_bit_products():
     run_distributed(_worker_vit, 1, backend="nccl")
+
+
+# ----------------------------------------------------------------------------- saved-tensor hooks
+def _spread(t):
+    """The same values at other strides: every second row of a wider buffer."""
+    if t.dim() == 0:
+        return t
+    raw = t.contiguous().view(torch.uint8) if t.element_size() == 1 else t.contiguous()
+    buffer = raw.new_zeros(*(2 * n for n in raw.shape))
+    view = buffer[tuple(slice(0, n) for n in raw.shape)] if t.dim() > 1 else buffer[::2]
+    view.copy_(raw)
+    return view.view(t.dtype) if t.element_size() == 1 else view
+
+
+@pytest.mark.parametrize("name", ["linear", "norm linear", "norm"])
+def test_what_saved_tensor_hooks_give_back(name):
+    """Copies at other strides give the same gradients; a tensor on another device, of another type or shape is refused."""
+    hooks = torch.autograd.graph.saved_tensors_hooks
+    inputs, f = _calls(130)[name]
+    leaves = [t.clone().requires_grad_() for t in inputs]
+    gs = [_tensor(*y.shape, seed=20 + k) for k, y in enumerate(f(*inputs))]
+    want = torch.autograd.grad(f(*leaves), leaves, gs)
+
+    def grads(unpack):
+        with hooks(lambda t: t.clone(), unpack):
+            outs = f(*leaves)
+        return torch.autograd.grad(outs, leaves, gs)
+
+    for unpack in (lambda t: t, _spread):
+        assert all(torch.equal(a, b) for a, b in zip(grads(unpack), want))
+    with torch.autograd.graph.save_on_cpu():
+        outs = f(*leaves)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(outs, leaves, gs), want))
+    for unpack in (lambda t: t.cpu(), lambda t: t.view(torch.uint8), lambda t: t[..., :-1], lambda t: t[:1], lambda t: t.double()):
+        with pytest.raises(RuntimeError):
+            grads(unpack)
