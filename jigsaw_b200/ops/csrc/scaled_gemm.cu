@@ -771,11 +771,13 @@ extern "C" int jb_scaled_gemm(const JbScaledOperand* a, const JbScaledOperand* b
   g.vec_out = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (ldo * size) % 16 == 0;
   const int M = a->rows, N = b->rows;
 #define JB_SG(BQ, PAIR) return launch_scaled_gemm<BQ, PAIR, false, false>(a->codes, a->pitch, b->codes, b->pitch, K, g, 1, sm_count, status, st)
+  // Up to 64 rows the weight lies along the lanes.  8192 x 4096: 10.6 us for one row, against 13.9 us in tiles of 128 rows, and
+  // 13.2 us both ways for 64 rows.
   if (M <= 64) {
     g.p = ob; g.q = oa;
     // How many CTAs share a tile: the one of 1, 2, 4, 8 with the least of (k-blocks of a CTA, 0.17 us each, or reading the
-    // weight at 6.5 TB/s) and the meeting of the parts (2 us).  Measured, one token: 1024 x 4096 takes 9.8 us whole and 6.2 us
-    // in eight parts, 8192 x 4096 10.1 us whole and 10.5 us in two.
+    // weight at 6.5 TB/s) and the meeting of the parts (2 us).  Measured, one token: 1024 x 4096 takes 9.9 us whole, 8.5, 7.1
+    // and 6.2 us in two, four and eight parts, 8192 x 4096 10.7 us whole and 12.2 us in two.
     const int tiles = (N + 127) / 128;
     const float memory = static_cast<float>(N) * static_cast<float>(K) / 6.5e6f;
     int split = 1;
@@ -795,19 +797,21 @@ extern "C" int jb_scaled_gemm(const JbScaledOperand* a, const JbScaledOperand* b
   g.p = oa; g.q = ob;
   // Tile width.  One k-block costs a CTA about 720 cycles at 128 x 256 and 600 at 128 x 128 (shared memory, which the loads
   // fill and the products read, is the bound of both), so the wide tile wins unless it leaves a wave of SMs idle:
-  // 4096 x 1024 x 4096 takes 16.9 us wide and 22.7 us narrow, 512 x 4096 x 4096 16 us and 13.5 us.
+  // 4096 x 1024 x 4096 takes 18.5 us wide and 24.9 us narrow, 512 x 4096 x 4096 17.8 us and 15.0 us.
   const long long tiles256 = static_cast<long long>((M + 127) / 128) * ((N + 255) / 256);
   const long long tiles128 = static_cast<long long>((M + 127) / 128) * ((N + 127) / 128);
   const long long waves256 = (tiles256 + sm_count - 1) / sm_count, waves128 = (tiles128 + sm_count - 1) / sm_count;
   if (waves256 * 720 <= waves128 * 600) {
-    // Pairs load a third less and run longer at higher clocks under the power limit (8192^3: 369 us against 430), but their
-    // hand-overs cost short products two microseconds (4096 x 4096 x 1024: 23.6 us against 21.0).
+    // Pairs load a third less, which pays where rows and waves are long, and costs short products up to two microseconds of
+    // hand-overs.  Pair and single CTA: 8192^3 395 and 426 us (after seconds of it, under the power limit at 1.1 to 1.2 GHz, 470
+    // and 498), 8192 x 11008 x 4096 278 and 295, 4096 x 4096 x 8192 105 and 110, x 2048 33.2 and 33.6, x 1024 25.3 and 22.9;
+    // a single wave: 4096 x 1024 x 4096 20.0 and 18.5, 2048 x 4096 x 4096 31.5 and 32.1.
     if (g.kblocks >= 16 && tiles256 >= 2LL * sm_count) { JB_SG(256, true); }
     JB_SG(256, false);
   }
   // A tile shared by a cluster costs 4 us (two CTAs) to 5 us (four) for the meeting of its parts, a k-block 0.26 us:
-  // 256 x 1024 x 8192 takes 20.9 us whole and 13.2 us in four parts (K = 4096: 12.6 and 11.2), 1024 x 1024 x 8192 21.2 us whole
-  // and 17.5 us in two (K = 4096: 12.9 and 13.3).
+  // 256 x 1024 x 8192 takes 21.3 us whole, 17.4 in two parts and 14.0 us in four (K = 4096: 12.8, 12.8 and 11.3),
+  // 1024 x 1024 x 8192 22.5 us whole and 19.3 us in two (K = 4096: 13.6 and 14.1).
   const int split = tiles128 * 4 <= sm_count && g.kblocks >= 32 ? 4 : tiles128 * 2 <= sm_count && g.kblocks >= 40 ? 2 : 1;
   if (split > 1) return launch_scaled_gemm<128, false, false, true>(a->codes, a->pitch, b->codes, b->pitch, K, g, split, sm_count, status, st);
   JB_SG(128, false);

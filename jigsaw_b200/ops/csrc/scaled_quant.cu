@@ -249,9 +249,10 @@ constexpr int quant_tile_smem() { return QT_SHARED + (MODE == QT_AHEAD ? 2 * 128
 // Tiles of 128 x 128, 32 values a thread (warp w: rows 8 w .. 8 w + 7, lane l: columns 4 l .. 4 l + 3).  Scales by row come
 // from warp reductions, by column through shared memory, or from the whole tile; the transposed codes turn in shared
 // memory, eight bytes of a column at a time.  A CTA takes tiles in steps of the grid; of 16-bit values it has the next tile
-// copied into shared memory while it works on the present one (8192 x 11008 bf16, both layouts: 134 us with loads, which
-// the warps waited for half of the time).  Two fp32 tiles ahead would leave room for one CTA an SM, which was slower
-// than loads (11001 x 4100: 48 us against 42; now 39).
+// copied into shared memory while it works on the present one (8192 x 11008 bf16, both layouts: that step took 134 us, half
+// of it waiting for loads, to 82; 72 us now).  Two fp32 tiles ahead would leave room for one CTA an SM, which was slower than
+// loads (11001 x 4100: 48 us against 42 at that time, 40 now).  16-bit rows that are not on 16-byte boundaries are read
+// element by element: 8192 x 4100 in squares takes 48 us, 8192 x 4096 18.
 template <typename T, int MODE, bool NORM>
 __global__ void __launch_bounds__(512, 2) quant_tile_kernel(const QuantArgs a, int tiles_r, int tiles) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -647,8 +648,10 @@ __global__ void __launch_bounds__(MOST) rms_fwd_kernel(const RmsArgs a) {
 
 // dx = r (w g - t r^2 mean(w g t)) + gsum and the gain's gradient sum_rows g t r.  A CTA takes rows in steps of the grid
 // and keeps the gain's partial sums of its columns in registers until the end; column_sum_kernel adds the CTAs' parts in
-// a fixed order.  The next row is read before the present one is worked on: with one row in flight the pass waited for
-// memory most of the time (16384 x 4096 bf16: 230 us, against 82 us of traffic).
+// a fixed order.  The next row is read before the present one is worked on.  For rows that the ring below does not take: off
+// 16-byte boundaries, where elements are loaded one by one (16384 x 4095 bf16: 308 us, 82 of traffic; 16384 x 4100, one larger
+// CTA an SM: 508), and rows too long for it (4096 x 20000 bf16, 64 registers a thread: 786 us, 100 of traffic; 8192 x 16384
+// fp32: 864, 327 of traffic).
 struct RmsBwdArgs {
   const void* t;             // the normalised sum, contiguous rows ldt apart
   long long ldt;
@@ -736,8 +739,9 @@ __global__ void __launch_bounds__(MOST, MOST <= 256 ? 2 : 1) rms_bwd_kernel(cons
 
 // The same pass with the rows brought into shared memory by bulk copies several batches ahead, for rows on 16-byte
 // boundaries.  A row belongs to `team` warps (8 NV values a thread), a batch is the `batch` rows that fit a CTA's eight or
-// sixteen; two CTAs of eight an SM cover one another's reductions (16384 x 4096 bf16: 119 us with direct loads).  The row is read from shared memory twice (for the sums, then for the gradient), so a thread keeps only the gain and its
-// partial sums, which the teams of a CTA add up at the end: one row of `part` a CTA.
+// sixteen; two CTAs of eight an SM cover one another's reductions (16384 x 4096 bf16: 100 us; 119 with direct wide loads, when
+// those took such rows).  The row is read from shared memory twice (for the sums, then for the gradient), so a thread keeps
+// only the gain and its partial sums, which the teams of a CTA add up at the end: one row of `part` a CTA.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
@@ -909,7 +913,7 @@ static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t
 static inline int rms_threads(int cols, int held) { return ((cols + held - 1) / held + 31) / 32 * 32; }
 
 // Rows of up to 1024 values: a warp each.  Longer ones: a CTA each, 32 values a thread, or 8 where there are fewer rows
-// than SMs and the time is that of one row's chain of loads and sums (4096 bf16, one row: 4.5 us with 32 a thread).
+// than SMs and the time is that of one row's chain of loads and sums (4096 bf16, one row: 4.5 us with 32 a thread, 2.5 with 8).
 template <typename T, bool VEC, bool CODES>
 static int launch_rms_fwd(const RmsArgs& a, int sm_count, cudaStream_t st) {
   const int warps = (a.rows + 7) / 8;
