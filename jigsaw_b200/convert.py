@@ -192,8 +192,8 @@ def convert_to_jigsaw(
     slice the same global weights.  Nothing is modified if the pre-flight check fails."""
     if on_unrecognized not in ("warn", "raise", "ignore"):
         raise ValueError(f"on_unrecognized must be 'warn', 'raise' or 'ignore', got {on_unrecognized!r}")
-    col_size = process_mesh_dict[col_kw].size() if col_kw in process_mesh_dict else 1
-    plan = ConversionPlan(model, convert_layer_norm, col_size)
+    col = process_mesh_dict[col_kw] if col_kw in process_mesh_dict else None
+    plan = ConversionPlan(model, convert_layer_norm, 1 if col is None else col.size())
     blocked = plan.findings("block")
     if blocked and not non_safe:
         raise ValueError(

@@ -106,3 +106,14 @@ def _worker_convert(rank, world):
         assert isinstance(layer, DistributedRMSNorm)
         for m in (layer, ref, layer.convert_to_torch(mesh)):
             assert all_ok(bool(((m(x).detach().double() - want).abs() <= 2 * _bound(want, dtype)).all()))
+
+
+@pytest.mark.parametrize("kind", [torch.nn.LayerNorm, torch.nn.RMSNorm])
+def test_norms_convert_without_groups(kind):
+    """A mesh whose axes have no group is a single process: nothing is cut."""
+    from jigsaw_b200 import convert
+
+    layer = convert.convert_to_jigsaw(kind(8), {"row": None, "col": None, "model": None}, "cpu")
+    assert type(layer).__name__ == f"Distributed{kind.__name__}" and layer.local_dim == 8
+    x = _rows(3, 8, dtype=torch.float32, size=1.0)
+    torch.testing.assert_close(layer(x), kind(8)(x))
